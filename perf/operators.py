@@ -132,8 +132,8 @@ def _run_capacity(tokens, requests, page):
 #
 # A page holds, per key/value head, page_tokens / 16 groups of 16 tokens, each
 # 16 * d key codes, then 16 * d value codes:
-#   key    [d/64][token / 8][token % 8][4][16]   feature = 64 a + 16 b + c
-#   value  [d/32][8][4][4][2][2]                 feature = 32 a + 4 b + d', token = 8 e + 2 c + f
+#   key    [j d/64][h 2][g 8][t 4][e 16]         feature = 64 j + 16 t + e, token = 8 h + g
+#   value  [j d/32][g 8][t 4][i 4][h 2][e 2]     feature = 32 j + 4 g + i, token = 8 h + 2 t + e
 # int8 codes are stored with 128 added, e4m3 codes as they are.
 
 def _to_layout(codes):
@@ -350,9 +350,10 @@ def _plain_append(state):
     ratio = _quotient(old, scale)[..., None, None]
     again = _to_codes(_code_values(raw, fmt) * ratio, fmt)
     again = torch.where(ratio == 1.0, raw, again)
-    zero = 128 if fmt == "int8" else 0
+    # rows behind the run: cleared by a run that begins its page, else left as they were
+    behind = torch.where((at > 0)[:, None, None, :, None], raw, 128 if fmt == "int8" else 0)
     written = _to_codes(_quotient(x, scale[..., None, None]), fmt)
-    codes = torch.where(fresh, written, torch.where(kept, again, zero)).to(torch.uint8)
+    codes = torch.where(fresh, written, torch.where(kept, again, behind)).to(torch.uint8)
     state["codes"][touched] = _to_layout(codes)
     state["scales"][touched] = scale
     return {"values": _code_values(codes, fmt) * scale[..., None, None], "scales": state["scales"]}
@@ -493,7 +494,8 @@ def _exact_append(state):
         ratio = (old / scale).float().double()[..., None, None]
         again = torch.where(ratio == 1, codes[:, :, side], _exact_round(codes[:, :, side] * ratio, fmt))
         fresh = _exact_round(x / scale[..., None, None], fmt)
-        code = torch.where(brings, fresh, torch.where(keeps, again, 0.0))
+        rest = codes[:, :, side] * (at > 0)[:, None, None, None]
+        code = torch.where(brings, fresh, torch.where(keeps, again, rest))
         values[:, :, side] = (code * scale[..., None, None]).float().double()
         scales[touched, :, side] = scale
     return {"values": values, "scales": scales}
