@@ -1,7 +1,7 @@
 /*
  * kq_b200 — B200-specific additions to the Kestrel-Q operator ABI.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *
  *  1. Reference internals that the reference's layer code calls and that a
  *     drop-in therefore has to export (declared in Kestrel-Q's
@@ -24,6 +24,9 @@
  *
  *  3. Asynchronous batched decode over device buffers, the serving path that
  *     the reference (batch 1, synchronous) has no counterpart for.
+ *
+ *  4. A paged 8-bit key/value cache for ragged batches of requests, with the
+ *     attention that reads it; no counterpart in the reference.
  *
  * Threading: every entry point takes a per-device lock; calls are ordered on
  * one CUDA stream per device (kq_b200_set_stream replaces it).
@@ -558,6 +561,172 @@ uint64_t kq_b200_kernel_launch_count(void);
  * the totals; kq_b200_profile_read waits for the recorded events. */
 void kq_b200_profile_kernel(const char *kernel_family);
 void kq_b200_profile_read(uint64_t *launches, double *total_ms);
+
+/* ---------------------------------------------------------------- group 4 */
+
+/* A key/value cache of pages shared by many requests.  A page holds
+ * `page_tokens` consecutive tokens of one request: their keys and values for
+ * every key/value head as 8-bit codes, with one F32 scale per (page, head,
+ * key or value); a value is code * scale.  The caller owns all memory (its
+ * own allocator, a fixed budget, a pool shared by layers); the library keeps
+ * nothing between calls and allocates nothing in them, so every call can be
+ * captured into a CUDA graph.
+ *
+ * A step brings new tokens of `request_count` requests: decode tokens, prompt
+ * chunks, or both.
+ *   kq_b200_kv8_plan    lengths -> query offsets, slots, positions, pages
+ *   kq_b200_kv8_append  quantises the new keys and values into their pages
+ *   kq_b200_kv8_attend  causal attention of the new tokens over the pages
+ *   kq_b200_kv8_read    the values that pages hold
+ *
+ * All arrays are device memory of the current device.  The calls are
+ * asynchronous on the library stream; what is wrong in the arrays' contents
+ * (lengths, page ids and slots out of range: KQ_STATUS_SPAN_OUT_OF_RANGE;
+ * non-finite values: KQ_STATUS_NUMERIC_DOMAIN) surfaces at
+ * kq_b200_synchronize, and nothing is read or written out of range meanwhile.
+ * After such an error the outputs of the failing call, and of the calls after
+ * it up to the synchronize, are unspecified; pages that a failed append met
+ * hold either their old rows or the new ones. */
+typedef enum kq_b200_kv8_format {
+    KQ_B200_KV8_INT8 = 0, /* -127 .. 127 */
+    KQ_B200_KV8_E4M3      /* 8-bit float, largest value 448 */
+} kq_b200_kv8_format;
+
+typedef enum kq_b200_kv8_dtype {
+    KQ_B200_KV8_F32 = 0,
+    KQ_B200_KV8_BF16
+} kq_b200_kv8_dtype;
+
+typedef struct kq_b200_kv8_cache {
+    uint32_t kv_head_count;
+    uint32_t head_dimension; /* 64, 128 or 256 */
+    uint32_t page_tokens;    /* 16, 32, 64 or 128 */
+    uint32_t page_count;
+    kq_b200_kv8_format format;
+    void *codes;             /* kq_b200_kv8_codes_bytes() bytes, 16-byte aligned */
+    uint64_t codes_bytes;
+    float *scales;           /* kq_b200_kv8_scales_count() values [page][head][key, value] */
+    uint64_t scales_count;
+} kq_b200_kv8_cache;
+
+/* Inside a page, per head, groups of 16 tokens follow each other, each
+ * 16 * d key codes, then 16 * d value codes, in the order that the
+ * attention's tensor-core operands read them (indexes slowest first):
+ *   key    [j: d/64][h: 2][g: 8][t: 4][e: 16]
+ *          feature 64 j + 16 t + e, token 8 h + g
+ *   value  [j: d/32][g: 8][t: 4][i: 4][h: 2][e: 2]
+ *          feature 32 j + 4 g + i, token 8 h + 2 t + e
+ * An int8 code is stored with 128 added.  0 if the geometry is not
+ * supported. */
+uint64_t kq_b200_kv8_codes_bytes(const kq_b200_kv8_cache *cache);
+uint64_t kq_b200_kv8_scales_count(const kq_b200_kv8_cache *cache);
+
+/* The arrays of one step.  kq_b200_kv8_plan fills all but the capacities;
+ * rows of the token arrays at and behind query_offsets[request_count] are
+ * padding (a step captured for a larger batch). */
+typedef struct kq_b200_kv8_step {
+    uint32_t request_count;   /* 1 .. 16384 */
+    uint32_t token_capacity;  /* rows of the step's token arrays */
+    uint32_t table_columns;   /* pages a request can have */
+    uint32_t run_capacity;    /* kq_b200_kv8_run_capacity() or more */
+    uint64_t table_stride;    /* entries between rows of block_table */
+    int32_t *block_table;     /* [request][column] page ids */
+    int32_t *query_offsets;   /* [request_count + 1] first new token of each request */
+    int32_t *kv_lengths;      /* [request_count] cached tokens, the new ones included */
+    int64_t *slots;           /* [token_capacity] page * page_tokens + row; -1 behind the last token */
+    int32_t *positions;       /* [token_capacity] position in the request; -1 behind the last token */
+    int32_t *run_offsets;     /* [request_count + 1] first page run of each request */
+    int32_t *page_runs;       /* [run_capacity] first new token of each (request, page); -1 behind the last */
+} kq_b200_kv8_step;
+
+/* The most (request, page) runs of a step: min(tokens, tokens / page_tokens
+ * + 2 * requests). */
+uint64_t kq_b200_kv8_run_capacity(uint32_t tokens, uint32_t requests, uint32_t page_tokens);
+
+/* Builds the step from the requests' lengths: `context_lengths` [requests]
+ * tokens cached before, `new_lengths` [requests] new tokens (both may be 0).
+ * Pages that a request enters are taken, in request order, from
+ * free_pages[*free_head ...] (`free_count` ids) and written into its row of
+ * step->block_table, whose other entries stay as they are; *free_head_out
+ * = *free_head + pages taken.  A step that needs more pages, columns, tokens
+ * or runs than there are writes nothing.  free_head_out must not be
+ * free_head, nor step->kv_lengths the context lengths: the same step can be
+ * planned again. */
+kq_status kq_b200_kv8_plan(const kq_b200_kv8_cache *cache,
+                           const kq_b200_kv8_step *step,
+                           const int32_t *context_lengths,
+                           const int32_t *new_lengths,
+                           const int32_t *free_pages,
+                           uint32_t free_count,
+                           const int32_t *free_head,
+                           int32_t *free_head_out,
+                           kq_diagnostic *diagnostic);
+
+/* Quantises the rows key / value [token_capacity][kv heads][d] (`key_stride`,
+ * `value_stride` elements between tokens, rows 16-byte aligned) into the
+ * slots of step->page_runs.  A page's scale is the largest magnitude it has
+ * held divided by 127 (int8) or 448 (e4m3): where new rows exceed it, the
+ * rows before them are rounded again to the new scale.  A run that begins at
+ * a page's first row starts the page anew and clears the rows behind it; rows
+ * behind a run that begins later stay as they are.  Non-finite rows leave
+ * their page as it was.  The runs of a call must lie in different pages (as
+ * kq_b200_kv8_plan makes them): what two runs in one page leave there is
+ * unspecified. */
+kq_status kq_b200_kv8_append(const kq_b200_kv8_cache *cache,
+                             const kq_b200_kv8_step *step,
+                             kq_b200_kv8_dtype dtype,
+                             const void *key,
+                             uint64_t key_stride,
+                             const void *value,
+                             uint64_t value_stride,
+                             kq_diagnostic *diagnostic);
+
+/* The values of `count` pages (ids in device memory, any order, repeats
+ * allowed) as F32 [count][kv heads][key, value][page_tokens][d]. */
+kq_status kq_b200_kv8_read(const kq_b200_kv8_cache *cache,
+                           const int32_t *pages,
+                           uint32_t count,
+                           float *values,
+                           uint64_t values_capacity,
+                           kq_diagnostic *diagnostic);
+
+/* Work space that kq_b200_kv8_attend needs for these sizes (0: none). */
+kq_status kq_b200_kv8_attend_workspace_bytes(const kq_b200_kv8_cache *cache,
+                                             const kq_b200_kv8_step *step,
+                                             uint32_t query_heads,
+                                             uint64_t max_kv_length,
+                                             uint64_t *bytes,
+                                             kq_diagnostic *diagnostic);
+
+/* Attention of the step's tokens: token i of request b (row query_offsets[b]
+ * + i of `query` and `output`, [token][query heads][d], `*_stride` elements
+ * between tokens, rows 16-byte aligned) sees the cached tokens up to its
+ * position kv_lengths[b] - new tokens + i; query head h reads key/value head
+ * h / (query heads / kv heads).
+ *   output = softmax(softmax_scale * q . k) v,   lse = log sum exp of the logits
+ * (natural logarithm, [token][query heads], may be NULL).  A row that sees
+ * nothing gets zeros and -infinity; rows behind the last request are left as
+ * they were.  Uses step->block_table, query_offsets and kv_lengths only.
+ * Query and output have the same type; products are exact in the codes and
+ * hold 22 bits of an F32 query, sums and the softmax are F32.
+ * `max_kv_length` (0: what the table's columns hold) and the capacities only
+ * decide how the work is cut; the result is right for any lengths, and the
+ * same for the same cut.  `workspace` is private to the call until it has
+ * completed: graphs that may run at the same time need one each. */
+kq_status kq_b200_kv8_attend(const kq_b200_kv8_cache *cache,
+                             const kq_b200_kv8_step *step,
+                             kq_b200_kv8_dtype dtype,
+                             const void *query,
+                             uint64_t query_stride,
+                             uint32_t query_heads,
+                             float softmax_scale,
+                             uint64_t max_kv_length,
+                             void *output,
+                             uint64_t output_stride,
+                             float *lse,
+                             void *workspace,
+                             uint64_t workspace_bytes,
+                             kq_diagnostic *diagnostic);
 
 #ifdef __cplusplus
 }

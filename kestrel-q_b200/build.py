@@ -33,6 +33,8 @@ SOURCES = [
     "kernels_umma.cu",
     "kernels_moe.cu",
     "kernels_layer.cu",
+    "kernels_kv8.cu",
+    "kernels_kv8_attend.cu",
     "runtime.cpp",
     "api_basic.cpp",
     "api_provider.cpp",
@@ -40,6 +42,7 @@ SOURCES = [
     "api_qsa.cpp",
     "api_moe.cpp",
     "api_layer.cpp",
+    "api_kv8.cpp",
     "api_static.cu",
 ]
 

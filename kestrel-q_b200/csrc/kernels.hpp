@@ -71,6 +71,7 @@ enum DeviceError : uint32_t {
     kErrSelection = 3,   // QSA selected-token count invalid
     kErrTimeout = 4,     // a bounded wait gave up (wait site in bits 8..15)
     kErrRange = 5,       // an activation beyond the tensor-core projection's range (|x| >= 2^18)
+    kErrStep = 6,        // a paged-cache step whose lengths, pages or offsets are out of range
 };
 
 // One quantized (or F32/BF16) matrix in HBM: `rows` consecutive GGUF rows.

@@ -154,6 +154,7 @@ static const char *error_text(uint32_t code) {
     case kErrSelection: return "QSA selected-token count is invalid";
     case kErrTimeout: return "a tensor-core pipeline wait that timed out";
     case kErrRange: return "a projection input is beyond the tensor-core range (|x| >= 2^18)";
+    case kErrStep: return "a paged-cache step whose lengths, pages or offsets are out of range";
     default: return "device error";
     }
 }
@@ -174,7 +175,9 @@ kq_status DeviceContext::synchronize(kq_diagnostic *d) {
         for (Rollbackable *r : dirty) r->on_error(failing);
         dirty.clear();
         KQB_CUDA(cudaMemsetAsync(err_word, 0, sizeof(unsigned long long), stream), d, "error word reset");
-        kq_status s = code == kErrSelection ? KQ_STATUS_INVALID_QSA_STATE : KQ_STATUS_NUMERIC_DOMAIN;
+        kq_status s = code == kErrSelection ? KQ_STATUS_INVALID_QSA_STATE
+                      : code == kErrStep    ? KQ_STATUS_SPAN_OUT_OF_RANGE
+                                            : KQ_STATUS_NUMERIC_DOMAIN;
         diag_set(d, s, "device reported %s (code 0x%x, call %u); state rolled back", error_text(code), code,
                  failing);
         return s;

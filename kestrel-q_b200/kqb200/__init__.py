@@ -17,7 +17,7 @@ from . import abi, synth
 from .abi import KQError, lib
 
 __all__ = ["abi", "synth", "lib", "KQError", "Provider", "GdnLayer", "GdnState", "QsaLayer",
-           "QsaState", "build"]
+           "QsaState", "Kv8Cache", "Kv8Step", "build"]
 
 
 def build(force: bool = False):
@@ -576,6 +576,145 @@ def qsa_prefill_sharded_async(state: QsaState, x_ptr: int, tokens: int, y_ptr: i
     d = abi.Diagnostic()
     abi.check(lib().kq_b200_qsa_prefill_split_async(state.layer.handle, state.handle, x_ptr, tokens, y_ptr, rank,
                                                     world, token_part, token_parts, exchange, None, C.byref(d)), d)
+
+
+class Kv8Step:
+    """The device arrays of one step of a paged cache (kq_b200_kv8_step):
+    `requests` rows of `block_table` (int32 [requests][columns], the caller's),
+    token arrays of `tokens` rows.  :meth:`Kv8Cache.plan` fills them;
+    :meth:`use` puts a caller's own in their place."""
+
+    _TYPES = {"query_offsets": "int32", "kv_lengths": "int32", "slots": "int64", "positions": "int32",
+              "run_offsets": "int32", "page_runs": "int32"}
+
+    def __init__(self, requests: int, tokens: int, block_table, page_tokens: int):
+        import torch
+        runs = max(1, lib().kq_b200_kv8_run_capacity(tokens, requests, page_tokens))
+        self.block_table = _tensor("block_table", block_table, "int32")
+        if block_table.dim() != 2 or block_table.shape[0] < requests or \
+                (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            raise ValueError("block_table: a row of page ids for every request is required")
+        self._sizes = {"query_offsets": requests + 1, "kv_lengths": requests, "slots": tokens, "positions": tokens,
+                       "run_offsets": requests + 1, "page_runs": runs}
+        self.args = abi.Kv8StepArgs(requests, tokens, block_table.shape[1], runs,
+                                    block_table.stride(0) if requests > 1 else block_table.shape[1],
+                                    block_table.data_ptr())
+        self.use(**{n: torch.empty(k, dtype=getattr(torch, self._TYPES[n]), device=block_table.device)
+                    for n, k in self._sizes.items()})
+
+    def use(self, **arrays) -> None:
+        for name, a in arrays.items():
+            _tensor(name, a, self._TYPES[name])
+            if a.numel() < self._sizes[name] or not a.is_contiguous():
+                raise ValueError(f"{name}: {self._sizes[name]} consecutive values are required")
+            setattr(self, name, a)
+            setattr(self.args, name, a.data_ptr())
+        if "page_runs" in arrays:
+            self.args.run_capacity = arrays["page_runs"].numel()
+
+
+class Kv8Cache:
+    """A paged 8-bit key/value cache (kq_b200_kv8_cache) over torch arrays:
+    `codes` (uint8) and `scales` (float32), allocated empty if not given.
+    The calls are asynchronous on the library stream."""
+
+    FORMATS = {"int8": 0, "e4m3": 1}
+
+    def __init__(self, kv_heads: int, head_dim: int, page_tokens: int, pages: int, format: str = "int8",
+                 codes=None, scales=None, device="cuda"):
+        import torch
+        self._dtypes = {torch.float32: 0, torch.bfloat16: 1}
+        self.kv_heads, self.head_dim, self.page_tokens, self.pages = kv_heads, head_dim, page_tokens, pages
+        self.args = abi.Kv8CacheArgs(kv_heads, head_dim, page_tokens, pages, self.FORMATS[format])
+        nbytes = lib().kq_b200_kv8_codes_bytes(C.byref(self.args))
+        count = lib().kq_b200_kv8_scales_count(C.byref(self.args))
+        if nbytes == 0:
+            raise ValueError("the cache's heads, head dimension or page size is not supported")
+        if codes is None:   # code 0 everywhere
+            codes = torch.full((nbytes,), 128 if format == "int8" else 0, dtype=torch.uint8, device=device)
+        if scales is None:
+            scales = torch.zeros(count, dtype=torch.float32, device=device)
+        self.codes, self.scales = _tensor("codes", codes, "uint8"), _tensor("scales", scales, "float32")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("cache arrays must be contiguous")
+        self.args.codes, self.args.codes_bytes = codes.data_ptr(), codes.numel()
+        self.args.scales, self.args.scales_count = scales.data_ptr(), scales.numel()
+
+    def _rows(self, name: str, a, tokens: int, heads: int | None):
+        """(dtype, address, token stride) of rows [tokens][heads][head_dim]
+        (the stride of a dimension of one element says nothing)."""
+        if a.dim() != 3 or a.shape[0] < tokens or a.shape[2] != self.head_dim or a.stride(2) != 1 \
+                or (a.shape[1] > 1 and a.stride(1) != self.head_dim) or (heads is not None and a.shape[1] != heads):
+            raise ValueError(f"{name}: rows [tokens][heads][{self.head_dim}] with consecutive heads are required")
+        if a.dtype not in self._dtypes:
+            raise ValueError(f"{name}: float32 or bfloat16 is required")
+        return self._dtypes[a.dtype], a.data_ptr(), a.stride(0) if tokens > 1 else a.shape[1] * self.head_dim
+
+    def plan(self, step: Kv8Step, context_lengths, new_lengths, free_pages, free_head, free_head_out) -> None:
+        n = step.args.request_count
+        for name, a, least in (("context_lengths", context_lengths, n), ("new_lengths", new_lengths, n),
+                               ("free_pages", free_pages, 0), ("free_head", free_head, 1),
+                               ("free_head_out", free_head_out, 1)):
+            _tensor(name, a, "int32")
+            if a.numel() < least or not a.is_contiguous():
+                raise ValueError(f"{name}: {least} consecutive values are required")
+        d = abi.Diagnostic()
+        abi.check(lib().kq_b200_kv8_plan(self.args, step.args, context_lengths.data_ptr(), new_lengths.data_ptr(),
+                                         free_pages.data_ptr(), free_pages.numel(), free_head.data_ptr(),
+                                         free_head_out.data_ptr(), C.byref(d)), d)
+
+    def append(self, step: Kv8Step, key, value) -> None:
+        n = step.args.token_capacity
+        kt, kp, ks = self._rows("key", key, n, self.kv_heads)
+        vt, vp, vs = self._rows("value", value, n, self.kv_heads)
+        if kt != vt:
+            raise ValueError("key and value must have the same type")
+        d = abi.Diagnostic()
+        abi.check(lib().kq_b200_kv8_append(self.args, step.args, kt, kp, ks, vp, vs, C.byref(d)), d)
+
+    def read_pages(self, pages, values) -> None:
+        """values (float32 [pages][heads][key, value][page_tokens][head_dim]) of the page ids `pages` (int32)."""
+        _tensor("pages", pages, "int32")
+        _tensor("values", values, "float32")
+        if not (pages.is_contiguous() and values.is_contiguous()):
+            raise ValueError("pages and values must be contiguous")
+        d = abi.Diagnostic()
+        abi.check(lib().kq_b200_kv8_read(self.args, pages.data_ptr(), pages.numel(), values.data_ptr(), values.numel(),
+                                         C.byref(d)), d)
+
+    def attend_workspace_bytes(self, step: Kv8Step, query_heads: int, max_kv_length: int = 0) -> int:
+        n, d = C.c_uint64(), abi.Diagnostic()
+        abi.check(lib().kq_b200_kv8_attend_workspace_bytes(self.args, step.args, query_heads, max_kv_length, C.byref(n),
+                                                           C.byref(d)), d)
+        return n.value
+
+    def attend(self, step: Kv8Step, query, output, lse=None, *, scale: float, max_kv_length: int = 0,
+               workspace=None) -> None:
+        """Attention of `query` [tokens][query heads][head_dim] into `output`
+        (same type) and `lse` (float32 [tokens][query heads]).  `workspace`:
+        a contiguous array of attend_workspace_bytes()."""
+        n = step.args.token_capacity
+        qt, qp, qs = self._rows("query", query, n, None)
+        ot, op, os = self._rows("output", output, n, query.shape[1])
+        if qt != ot:
+            raise ValueError("query and output must have the same type")
+        if lse is not None:
+            _tensor("lse", lse, "float32")
+            if lse.numel() < n * query.shape[1] or not lse.is_contiguous():
+                raise ValueError("lse: one value per token and query head is required")
+        if workspace is not None and not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        d = abi.Diagnostic()
+        abi.check(lib().kq_b200_kv8_attend(self.args, step.args, qt, qp, qs, query.shape[1], scale, max_kv_length, op, os,
+                                           None if lse is None else lse.data_ptr(),
+                                           None if workspace is None else workspace.data_ptr(),
+                                           0 if workspace is None else workspace.nbytes, C.byref(d)), d)
+
+
+def _tensor(name: str, a, dtype: str):
+    if str(a.dtype) != "torch." + dtype:
+        raise ValueError(f"{name}: {dtype} is required")
+    return a
 
 
 def synchronize() -> None:

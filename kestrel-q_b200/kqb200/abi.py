@@ -20,6 +20,7 @@ OUT_OF_MEMORY = 2
 UNSUPPORTED_TENSOR_TYPE = 12
 ARITHMETIC_OVERFLOW = 13
 LIMIT_EXCEEDED = 14
+INVALID_ALIGNMENT = 15
 SPAN_OUT_OF_RANGE = 16
 UNSUPPORTED_MODEL = 20
 SEMANTIC_MAPPING_FAILED = 22
@@ -72,6 +73,17 @@ def _pair_fields(names):
     for n in names:
         out += [(n, vp), (n + "_count", u64)]
     return out
+
+
+class Kv8CacheArgs(C.Structure):
+    _fields_ = [("kv_head_count", u32), ("head_dimension", u32), ("page_tokens", u32), ("page_count", u32),
+                ("format", C.c_int), ("codes", vp), ("codes_bytes", u64), ("scales", vp), ("scales_count", u64)]
+
+
+class Kv8StepArgs(C.Structure):
+    _fields_ = [("request_count", u32), ("token_capacity", u32), ("table_columns", u32), ("run_capacity", u32),
+                ("table_stride", u64), ("block_table", vp), ("query_offsets", vp), ("kv_lengths", vp), ("slots", vp),
+                ("positions", vp), ("run_offsets", vp), ("page_runs", vp)]
 
 
 MOE_WEIGHT_FIELDS = ["router", "routed_gate", "routed_up", "routed_down", "shared_gate", "shared_up",
@@ -347,6 +359,16 @@ _SIGNATURES = {
                                                 vp, vp, vp]),
     "kq_b200_layer_decode_batch": (C.c_int, [vp, C.POINTER(vp), u32, vp, vp, vp]),
     "kq_b200_layer_prefill_async": (C.c_int, [vp, vp, vp, u64, vp, vp]),
+    "kq_b200_kv8_codes_bytes": (u64, [C.POINTER(Kv8CacheArgs)]),
+    "kq_b200_kv8_scales_count": (u64, [C.POINTER(Kv8CacheArgs)]),
+    "kq_b200_kv8_run_capacity": (u64, [u32, u32, u32]),
+    "kq_b200_kv8_plan": (C.c_int, [C.POINTER(Kv8CacheArgs), C.POINTER(Kv8StepArgs), vp, vp, vp, u32, vp, vp, vp]),
+    "kq_b200_kv8_append": (C.c_int, [C.POINTER(Kv8CacheArgs), C.POINTER(Kv8StepArgs), C.c_int, vp, u64, vp, u64, vp]),
+    "kq_b200_kv8_read": (C.c_int, [C.POINTER(Kv8CacheArgs), vp, u32, vp, u64, vp]),
+    "kq_b200_kv8_attend_workspace_bytes": (C.c_int, [C.POINTER(Kv8CacheArgs), C.POINTER(Kv8StepArgs), u32, u64,
+                                                     C.POINTER(u64), vp]),
+    "kq_b200_kv8_attend": (C.c_int, [C.POINTER(Kv8CacheArgs), C.POINTER(Kv8StepArgs), C.c_int, vp, u64, u32, f32, u64,
+                                     vp, u64, vp, vp, u64, vp]),
     "kq_layer_family_name": (C.c_char_p, [C.c_int]),
     "kq_layer_checkpoint_kind_name": (C.c_char_p, [C.c_int]),
     "kq_gdn_checkpoint_kind_name": (C.c_char_p, [C.c_int]),
