@@ -170,8 +170,18 @@ __device__ __forceinline__ bool load_request(const Kv8Cache &c, const Kv8Step &s
     return ok;
 }
 
-// One 16-row tile per warp and MT: softmax state and accumulators.
-// Thread (g, t) = (lane / 4, lane % 4) holds rows g and g + 8.
+// How a warp's 16 MMA rows are used:
+//   kPlain    16 query rows, fp16-exact queries (bfloat16)
+//   kTwoTerm  16 query rows, every product in two terms (F32)
+//   kStacked  8 query rows: rows 0-7 hold the high parts of Q and of the
+//             weights, rows 8-15 the low parts (F32), so that one product
+//             does both; the halves meet in the same thread's registers
+enum Mode { kPlain, kTwoTerm, kStacked };
+constexpr int terms_of(int mode) { return mode == kTwoTerm ? 2 : 1; }
+constexpr int rows_of(int mode) { return mode == kStacked ? 8 : 16; }
+
+// One tile per warp and MT: softmax state and accumulators.  Thread (g, t) =
+// (lane / 4, lane % 4) holds rows g and, except when stacked, g + 8.
 template <int D, int MT>
 struct Rows {
     float o[MT][D / 8][4];
@@ -196,58 +206,81 @@ struct Rows {
 // [MT][TERMS][D / 16][32 lanes].  factor: per row, softmax scale * log2 e /
 // the row's power of two.  limit: last visible token per row (-1: none);
 // compared only when MASK.
-template <int D, int MT, int NG, int TERMS, bool E4M3, bool MASK>
+// The first product's sums run in eight independent accumulators per thread
+// (CH chains per tile): a chain of D / 16 dependent MMAs per group was what
+// the row kernel waited for (302 us against 225 for 64 F32 sequences).
+template <int D, int MT, int NG, int MODE, bool E4M3, bool MASK>
 __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, const uint8_t *kv, const float (&ks)[NG],
                                            const float (&vs)[NG], const float (&factor)[MT][2],
                                            const int32_t (&limit)[MT][2], int32_t token, uint32_t lane) {
+    constexpr int TERMS = terms_of(MODE), R = MODE == kStacked ? 1 : 2;
+    constexpr int CH = MT * NG >= 4 ? 1 : 4 / (MT * NG);
     float s[MT][NG][2][4];
+    {
+        float c[CH][MT][NG][2][4];
 #pragma unroll
-    for (int a = 0; a < MT; ++a)
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[a][n][h][k] = 0.0f;
-
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-        uint4 w[NG][2];
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                w[n][h] = *reinterpret_cast<const uint4 *>(kv + n * 32 * D + j * 1024 + h * 512 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t b[NG][2][2];
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint4 &x = w[n][h];
-                    widen<E4M3>(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, b[n][h][0], b[n][h][1]);
-                }
+        for (int x = 0; x < CH; ++x)
 #pragma unroll
             for (int a = 0; a < MT; ++a)
 #pragma unroll
-                for (int term = TERMS - 1; term >= 0; --term) {
-                    const uint4 f = q[((a * TERMS + term) * (D / 16) + j * 4 + i) * 32 + lane];
+                for (int n = 0; n < NG; ++n)
 #pragma unroll
-                    for (int n = 0; n < NG; ++n)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) mma(s[a][n][h], f, b[n][h][0], b[n][h][1]);
-                }
+                        for (int k = 0; k < 4; ++k) c[x][a][n][h][k] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            uint4 w[NG][2];
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w[n][h] = *reinterpret_cast<const uint4 *>(kv + n * 32 * D + j * 1024 + h * 512 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t b[NG][2][2];
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 &x = w[n][h];
+                        widen<E4M3>(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, b[n][h][0], b[n][h][1]);
+                    }
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int term = TERMS - 1; term >= 0; --term) {
+                        const uint4 f = q[((a * TERMS + term) * (D / 16) + j * 4 + i) * 32 + lane];
+#pragma unroll
+                        for (int n = 0; n < NG; ++n)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                mma(c[(i * TERMS + term) % CH][a][n][h], f, b[n][h][0], b[n][h][1]);
+                    }
+            }
         }
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float v = c[0][a][n][h][k];
+#pragma unroll
+                        for (int x = 1; x < CH; ++x) v += c[x][a][n][h][k];
+                        s[a][n][h][k] = v;
+                    }
     }
 
     // logits, the rows' maxima
-    float top[MT][2];
+    float top[MT][R];
     bool lift = false;
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < R; ++r) {
             float x = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -256,7 +289,9 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float v = s[a][n][h][2 * r + k] * f;
+                        float v = s[a][n][h][2 * r + k];
+                        if constexpr (MODE == kStacked) v += s[a][n][h][2 + k];
+                        v *= f;
                         if (MASK && token + n * 16 + h * 8 + (int32_t)(lane & 3) * 2 + k > limit[a][r]) v = -INFINITY;
                         s[a][n][h][2 * r + k] = v;
                         x = fmaxf(x, v);
@@ -270,16 +305,21 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
     }
     if (__any_sync(~0u, lift)) {   // -inf + 8 is -inf: the first finite logit of a row lifts it
 #pragma unroll
-        for (int a = 0; a < MT; ++a)
+        for (int a = 0; a < MT; ++a) {
+            float by[2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < R; ++r) {
                 const float m = fmaxf(st.m[a][r], top[a][r]);
-                const float by = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
+                by[r] = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
                 st.m[a][r] = m;
-                st.l[a][r] *= by;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) st.o[a][n][2 * r] *= by, st.o[a][n][2 * r + 1] *= by;
+                st.l[a][r] *= by[r];
             }
+            if constexpr (R == 1) by[1] = by[0];
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by[k >> 1];
+        }
     }
     float most = vs[0];
 #pragma unroll
@@ -303,25 +343,33 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
     uint4 p[MT][NG][TERMS];
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
-        const float m0 = st.m[a][0] == -INFINITY ? 0.0f : st.m[a][0], m1 = st.m[a][1] == -INFINITY ? 0.0f : st.m[a][1];
+        float m[2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) m[r] = st.m[a][r] == -INFINITY ? 0.0f : st.m[a][r];
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             const float w = vs[n] * inv;
-            float e[2][4];
+            float e[2][2 * R];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    e[h][k] = exp2_approx(s[a][n][h][k] - (k < 2 ? m0 : m1));
+                for (int k = 0; k < 2 * R; ++k) {
+                    e[h][k] = exp2_approx(s[a][n][h][k] - m[k >> 1]);
                     st.l[a][k >> 1] += e[h][k];
                     e[h][k] *= w;
                 }
             }
-            p[a][n][0] = make_uint4(pack_half(e[0][0], e[0][1]), pack_half(e[0][2], e[0][3]), pack_half(e[1][0], e[1][1]),
-                                    pack_half(e[1][2], e[1][3]));
-            if constexpr (TERMS == 2)
-                p[a][n][1] = make_uint4(pack_rest(e[0][0], e[0][1], p[a][n][0].x), pack_rest(e[0][2], e[0][3], p[a][n][0].y),
-                                        pack_rest(e[1][0], e[1][1], p[a][n][0].z), pack_rest(e[1][2], e[1][3], p[a][n][0].w));
+            if constexpr (MODE == kStacked) {
+                const uint32_t h0 = pack_half(e[0][0], e[0][1]), h1 = pack_half(e[1][0], e[1][1]);
+                p[a][n][0] = make_uint4(h0, pack_rest(e[0][0], e[0][1], h0), h1, pack_rest(e[1][0], e[1][1], h1));
+            } else {
+                p[a][n][0] = make_uint4(pack_half(e[0][0], e[0][1]), pack_half(e[0][2], e[0][3]),
+                                        pack_half(e[1][0], e[1][1]), pack_half(e[1][2], e[1][3]));
+                if constexpr (TERMS == 2)
+                    p[a][n][1] =
+                        make_uint4(pack_rest(e[0][0], e[0][1], p[a][n][0].x), pack_rest(e[0][2], e[0][3], p[a][n][0].y),
+                                   pack_rest(e[1][0], e[1][1], p[a][n][0].z), pack_rest(e[1][2], e[1][3], p[a][n][0].w));
+            }
         }
     }
 
@@ -365,9 +413,10 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
 // factor and its last visible token into limit.  Eight threads per row, every
 // thread of the CTA takes part; rows behind the request's last are zero with
 // limit -1.  Returns whether a query value was not finite.
-template <int D, int TERMS, bool BF16, int THREADS, int ROWS>
+template <int D, int MODE, int THREADS, int ROWS>
 __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &rq, uint32_t G, uint32_t head,
                                              uint32_t row0, uint4 *q, float *factor, int32_t *limit, uint32_t tid) {
+    constexpr int TERMS = terms_of(MODE);
     bool bad = false;
     uint32_t *q32 = reinterpret_cast<uint32_t *>(q);
     const uint32_t part = tid & 7;
@@ -382,7 +431,7 @@ __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &
             if (live) {
                 const uint64_t at = (uint64_t)(rq.first + token) * a.q_stride + (uint64_t)(head * G + row % G) * D +
                                     (part + 8 * k) * 4;
-                if constexpr (BF16) {
+                if constexpr (MODE == kPlain) {
                     const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
                     v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
                                     __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
@@ -410,9 +459,10 @@ __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &
             const uint32_t h0 = pack_half(x[4 * k] * up, x[4 * k + 1] * up), h1 = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
             q32[at] = h0;
             q32[at + 2] = h1;
-            if constexpr (TERMS == 2) {
-                q32[at + D / 16 * 128] = pack_rest(x[4 * k] * up, x[4 * k + 1] * up, h0);
-                q32[at + D / 16 * 128 + 2] = pack_rest(x[4 * k + 2] * up, x[4 * k + 3] * up, h1);
+            if constexpr (MODE != kPlain) {
+                constexpr uint32_t low = MODE == kStacked ? 1 : D / 16 * 128;   // rows 8-15, or the second term
+                q32[at + low] = pack_rest(x[4 * k] * up, x[4 * k + 1] * up, h0);
+                q32[at + low + 2] = pack_rest(x[4 * k + 2] * up, x[4 * k + 3] * up, h1);
             }
         }
         if (part == 0) {
@@ -435,6 +485,18 @@ __device__ __forceinline__ void store4(void *out, uint64_t at, float4 v) {
     }
 }
 
+// Where the partials of a (tile, head) lie: O [split][row][D], and behind the
+// O of all `tiles`, (m, l) [row][split].
+struct Partials {
+    float *o;
+    float2 *ml;
+    __device__ __forceinline__ Partials(float *base, uint64_t tile, uint32_t splits, uint32_t rows, uint32_t dim,
+                                        uint64_t tiles) {
+        o = base + tile * splits * rows * dim;
+        ml = reinterpret_cast<float2 *>(base + tiles * splits * rows * dim) + tile * rows * splits;
+    }
+};
+
 // Groups of 16 tokens that the rows up to `last_row` of a request see.
 __device__ __forceinline__ uint32_t visible_groups(const Request &rq, uint32_t G, uint32_t rows_end) {
     const uint32_t token = (rows_end - 1) / G;   // the tile's last token
@@ -454,15 +516,16 @@ template <int D, int TERMS> constexpr uint32_t kRowSmem = kRowWarps * kRowStages
 
 }  // namespace
 
-// grid (request, tile, head, split); four warps, 16 rows.  Each warp streams
+// grid (request, tile, head, split); four warps, 16 or 8 rows.  Each warp streams
 // every fourth group of the split through its own ring; page ids and scales of
 // a warp's next 32 groups sit in its lanes.
 // Partials: [request][tile][head][split][16 rows][D], then (m, l) per row.
-template <int D, bool BF16, bool E4M3>
+template <int D, int MODE, bool E4M3>
 __global__ void __launch_bounds__(kRowWarps * 32, 2)
 kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr int TERMS = BF16 ? 1 : 2, ST = kRowStages<D>;
-    constexpr uint32_t kStage = 32 * D;
+    constexpr int ST = kRowStages<D>;
+    constexpr bool BF16 = MODE == kPlain;
+    constexpr uint32_t kStage = 32 * D, kRows = rows_of(MODE), kR = MODE == kStacked ? 1 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kRowWarps][ST];
     __shared__ float factor_s[16], merge_m[kRowWarps][16], merge_l[kRowWarps][16];
@@ -485,14 +548,14 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
     const uint32_t rows = (uint32_t)rows64;
     // a request of more tiles than the launch has is not split: its partials
     // would have no place
-    const uint32_t splits = (rows + 15) / 16 > shape.row_tiles ? 1u : shape.row_splits;
+    const uint32_t splits = (rows + kRows - 1) / kRows > shape.row_tiles ? 1u : shape.row_splits;
     const int32_t *table = s.table + (uint64_t)b * s.table_stride;
     const uint32_t per_page = c.page_tokens / kG;
     const uint64_t page_bytes = 2ull * c.page_tokens * D;
     uint32_t used = 0;   // ring slots used so far (waits go by it)
 
-    for (uint32_t tile = tile0; tile * 16 < rows; tile += shape.row_tiles) {
-        const uint32_t row0 = tile * 16, row_end = min(row0 + 16, rows);
+    for (uint32_t tile = tile0; tile * kRows < rows; tile += shape.row_tiles) {
+        const uint32_t row0 = tile * kRows, row_end = min(row0 + kRows, rows);
         const uint32_t groups = visible_groups(rq, G, row_end), each = split_groups(groups, shape.row_groups, splits, 1);
         const uint32_t g0 = split * each, g1 = min(g0 + each, groups);
         if (split > 0 && g0 >= groups) break;   // later tiles see more groups only when splits == 1
@@ -525,13 +588,13 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
         uint32_t issued = 0;
         for (; issued < min(mine, (uint32_t)ST); ++issued) issue(issued);
 
-        if (load_queries<D, TERMS, BF16, kRowWarps * 32, 16>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
+        if (load_queries<D, MODE, kRowWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
             raise(err, kErrNonFinite);
         __syncthreads();
         Rows<D, 1> st;
         st.clear();
-        const float factor[1][2] = {{factor_s[lane >> 2], factor_s[(lane >> 2) + 8]}};
-        const int32_t limit[1][2] = {{limit_s[lane >> 2], limit_s[(lane >> 2) + 8]}};
+        const float factor[1][2] = {{factor_s[lane >> 2], factor_s[(lane >> 2) + 8 * (kR - 1)]}};
+        const int32_t limit[1][2] = {{limit_s[lane >> 2], limit_s[(lane >> 2) + 8 * (kR - 1)]}};
         // every row of the tile sees the tokens up to its first token's
         const uint32_t clear_to = rq.length + 1 > rq.n ? rq.length - rq.n + row0 / G + 1 : 0u;
         bool ok = true;
@@ -548,10 +611,10 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
             const float ks[1] = {__shfl_sync(~0u, scales.x, i & 31)}, vs[1] = {__shfl_sync(~0u, scales.y, i & 31)};
             const uint32_t token = (g0 + warp + i * kRowWarps) * kG;
             const uint8_t *kv = ring + slot * kStage;
-            if (token + kG > clear_to || row_end < row0 + 16)
-                group_step<D, 1, 1, TERMS, E4M3, true>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
+            if (token + kG > clear_to || row_end < row0 + kRows)
+                group_step<D, 1, 1, MODE, E4M3, true>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
             else
-                group_step<D, 1, 1, TERMS, E4M3, false>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                group_step<D, 1, 1, MODE, E4M3, false>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
             __syncwarp();
             // refill only with groups whose page ids the lanes hold
             if (issued < mine && (issued & ~31u) == (i & ~31u)) issue(issued++);
@@ -565,13 +628,13 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
 
         // join the warps: (m, l) and O of each in its own ring
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < (int)kR; ++r) {
             st.l[0][r] += __shfl_xor_sync(~0u, st.l[0][r], 1);
             st.l[0][r] += __shfl_xor_sync(~0u, st.l[0][r], 2);
         }
         if ((lane & 3) == 0) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < (int)kR; ++r) {
                 merge_m[warp][(lane >> 2) + 8 * r] = st.m[0][r];
                 merge_l[warp][(lane >> 2) + 8 * r] = st.l[0][r];
             }
@@ -582,17 +645,23 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < (int)kR; ++r)
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = st.o[0][4 * j + i][2 * r + k];
+                        if constexpr (MODE == kStacked) x[i] += st.o[0][4 * j + i][2 + k];
+                        x[i] *= back;
+                    }
                     *reinterpret_cast<float4 *>(mo + ((lane >> 2) + 8 * r) * kPitch + j * 32 + (lane & 3) * 8 + 4 * k) =
-                        make_float4(st.o[0][4 * j][2 * r + k] * back, st.o[0][4 * j + 1][2 * r + k] * back,
-                                    st.o[0][4 * j + 2][2 * r + k] * back, st.o[0][4 * j + 3][2 * r + k] * back);
+                        make_float4(x[0], x[1], x[2], x[3]);
+                }
         __syncthreads();
         const bool whole = groups <= each;   // one split: the result itself
-        float *part = nullptr;
-        if (!whole)
-            part = a.workspace + ((((uint64_t)b * shape.row_tiles + tile) * c.heads + head) * shape.row_splits + split) * 16 * (D + 2);
+        const Partials part(a.workspace, ((uint64_t)b * shape.row_tiles + tile) * c.heads + head, shape.row_splits, 16, D,
+                            (uint64_t)s.requests * shape.row_tiles * c.heads);
         for (uint32_t v = tid; v < (row_end - row0) * (D / 4); v += kRowWarps * 32) {
             const uint32_t r = v / (D / 4), f = v % (D / 4) * 4;
             float m = merge_m[0][r];
@@ -618,8 +687,8 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
                 if (a.lse != nullptr && f == 0)
                     a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
             } else {
-                *reinterpret_cast<float4 *>(part + r * D + f) = o;
-                if (f == 0) *reinterpret_cast<float2 *>(part + 16 * D + 2 * r) = make_float2(m, l);
+                *reinterpret_cast<float4 *>(part.o + ((uint64_t)split * 16 + r) * D + f) = o;
+                if (f == 0) part.ml[r * shape.row_splits + split] = make_float2(m, l);
             }
         }
         if (__syncthreads_or(!ok)) return;
@@ -674,7 +743,7 @@ __device__ __forceinline__ uint32_t find_request(const Kv8Step &s, uint32_t G, u
 template <int D, bool BF16, bool E4M3>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr int TERMS = BF16 ? 1 : 2, MT = kPromptMt<D>, ST = kPromptStages<D>, NG = kPromptGroups;
+    constexpr int MODE = BF16 ? kPlain : kTwoTerm, TERMS = terms_of(MODE), MT = kPromptMt<D>, ST = kPromptStages<D>, NG = kPromptGroups;
     constexpr uint32_t kGroup = 32 * D, kStage = NG * kGroup, kRows = kPromptRows<D>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[ST], empty[ST];
@@ -752,7 +821,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
 
-    if (load_queries<D, TERMS, BF16, kPromptWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
+    if (load_queries<D, MODE, kPromptWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
         raise(err, kErrNonFinite);
     asm volatile("bar.sync 1, %0;" ::"n"(kPromptWarps * 32) : "memory");
     Rows<D, MT> st;
@@ -785,9 +854,9 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             const float ks[NG] = {s0.x, s1.x}, vs[NG] = {s0.y, s1.y};
             const uint8_t *kv = smem + slot * kStage;
             if (token + NG * kG > all_see || g0 + (k + 1) * NG > g1)
-                group_step<D, MT, NG, TERMS, E4M3, true>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                group_step<D, MT, NG, MODE, E4M3, true>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
             else
-                group_step<D, MT, NG, TERMS, E4M3, false>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                group_step<D, MT, NG, MODE, E4M3, false>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
         }
         __syncwarp();
         if (lane == 0) bar_arrive(&empty[slot]);
@@ -802,9 +871,8 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     if (!ok) return;
 
     const bool whole = groups <= each;
-    float *part = whole ? nullptr
-                        : a.workspace + shape.row_floats +
-                              (((uint64_t)t * c.heads + head) * shape.prompt_splits + split) * kRows * (D + 2);
+    const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, kRows, D,
+                        (uint64_t)shape.prompt_tiles * c.heads);
     const float back = st.ref * (1.0f / kWeightScale);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -829,12 +897,12 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                         fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
                         store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
                     } else {
-                        *reinterpret_cast<float4 *>(part + in_tile * D + f) = o;
+                        *reinterpret_cast<float4 *>(part.o + ((uint64_t)split * kRows + in_tile) * D + f) = o;
                     }
                 }
             if ((lane & 3) == 0) {
                 if (!whole)
-                    *reinterpret_cast<float2 *>(part + kRows * D + 2 * in_tile) = make_float2(st.m[m][r], l);
+                    part.ml[in_tile * shape.prompt_splits + split] = make_float2(st.m[m][r], l);
                 else if (a.lse != nullptr)
                     a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (st.m[m][r] + log2f(l)) * kLn2 : -INFINITY;
             }
@@ -842,18 +910,27 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         }
 }
 
-// Joins the splits of every split tile, in split order.  One CTA per (tile,
-// head, 16 rows); D / 4 threads per row.
+constexpr int kJoinThreads = 256;
+
+// Joins the splits of a row: one CTA per (tile, head, row), or per 64 features
+// of it where there are few.  The threads first turn the splits' (m, l) into
+// weights 2^(m_k - m) in shared memory, 1024 at a time; 16 threads then hold 4
+// features each of every 16th split, and meet in shared memory in a fixed
+// order.  Bound: latency, the partials come from L2.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinThreads)
 kv8_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, uint32_t prompt, ErrorWord err) {
-    // threads leave one by one (nothing below waits for the CTA), except
-    // that find_request needs its whole warp
-    const uint32_t lane = threadIdx.x & 31, G = a.query_heads / c.heads;
-    const uint32_t tile_rows = prompt ? shape.prompt_rows : 16u, blocks = tile_rows / 16;
-    const uint32_t block = blockIdx.x % blocks, u = blockIdx.x / blocks, head = u % c.heads, slot = u / c.heads;
+    constexpr uint32_t kLanes = 16, kWays = kJoinThreads / kLanes, kBatch = 1024, kAhead = 8;
+    __shared__ float weight[kBatch];
+    __shared__ float warp_red[kJoinThreads / 32];
+    __shared__ float4 way_sum[kWays][kLanes];
+    const uint32_t tid = threadIdx.x, lane = tid & 31, G = a.query_heads / c.heads;
+    const uint32_t tile_rows = prompt ? shape.prompt_rows : shape.join_rows;
+    const uint32_t chunks = prompt ? 1u : shape.join_chunks;
+    const uint32_t chunk = blockIdx.x % chunks, r0 = blockIdx.x / chunks % tile_rows;
+    const uint32_t u = blockIdx.x / chunks / tile_rows, head = u % c.heads, slot = u / c.heads;
     pdl_wait();
-    if (__syncthreads_or(threadIdx.x == 0 && err_raised(err))) return;
+    if (__syncthreads_or(tid == 0 && err_raised(err))) return;
     uint32_t b, tile;
     if (prompt) {
         uint32_t start;
@@ -867,41 +944,89 @@ kv8_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, uint32_t pro
     Request rq;
     if (!load_request(c, s, b, rq, err)) return;
     const uint64_t rows64 = (uint64_t)rq.n * G;
+    const uint32_t held = prompt ? shape.prompt_rows : shape.row_tile, pitch_rows = prompt ? shape.prompt_rows : 16u;
     if (prompt ? rows64 <= shape.row_limit : rows64 > shape.row_limit) return;
-    if (!prompt && (rows64 + 15) / 16 > shape.row_tiles) return;
-    if ((uint64_t)tile * tile_rows >= rows64) return;
-    const uint32_t rows = (uint32_t)rows64, row0 = tile * tile_rows, row_end = min(row0 + tile_rows, rows);
+    if (!prompt && (rows64 + held - 1) / held > shape.row_tiles) return;
+    if ((uint64_t)tile * held >= rows64) return;
+    const uint32_t rows = (uint32_t)rows64, row0 = tile * held, row_end = min(row0 + held, rows);
     const uint32_t launched = prompt ? shape.prompt_splits : shape.row_splits;
     const uint32_t groups = visible_groups(rq, G, row_end);
     const uint32_t each = split_groups(groups, prompt ? shape.prompt_groups : shape.row_groups, launched,
                                        prompt ? kPromptGroups : 1u);
     if (groups <= each) return;
     const uint32_t n = (groups + each - 1) / each;
-    const float *part = a.workspace + (prompt ? shape.row_floats : 0) +
-                        ((uint64_t)slot * c.heads + head) * launched * tile_rows * (D + 2);
-    for (uint32_t v = threadIdx.x; v < 16 * (D / 4); v += 256) {
-        const uint32_t r = block * 16 + v / (D / 4), f = v % (D / 4) * 4, row = row0 + r;
-        if (row >= row_end) break;
-        const float *ml = part + tile_rows * D + 2 * r, *po = part + r * D + f;
-        float m = -INFINITY;
-        for (uint32_t k = 0; k < n; ++k) m = fmaxf(m, ml[(uint64_t)k * tile_rows * (D + 2)]);
-        float l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (uint32_t k = 0; k < n; ++k) {
-            const float2 x = *reinterpret_cast<const float2 *>(ml + (uint64_t)k * tile_rows * (D + 2));
-            const float4 y = *reinterpret_cast<const float4 *>(po + (uint64_t)k * tile_rows * (D + 2));
-            const float by = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - m);
-            l += x.y * by;
-            o.x += y.x * by, o.y += y.y * by, o.z += y.z * by, o.w += y.w * by;
+    const Partials part(a.workspace + (prompt ? shape.row_floats : 0), (uint64_t)slot * c.heads + head, launched, pitch_rows,
+                        D, (uint64_t)(prompt ? shape.prompt_tiles : s.requests * shape.row_tiles) * c.heads);
+
+    auto all = [&](float v, bool take_max) {   // over the CTA, the same in every thread
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float x = __shfl_xor_sync(~0u, v, o);
+            v = take_max ? fmaxf(v, x) : v + x;
         }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-        if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY)) raise(err, kErrNonFinite);
-        const uint32_t token = rq.first + row / G, qh = head * G + row % G;
-        store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
-        if (a.lse != nullptr && f == 0)
-            a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        __syncthreads();
+        if (lane == 0) warp_red[tid >> 5] = v;
+        __syncthreads();
+        v = warp_red[0];
+#pragma unroll
+        for (int w = 1; w < kJoinThreads / 32; ++w) v = take_max ? fmaxf(v, warp_red[w]) : v + warp_red[w];
+        return v;
+    };
+    const uint32_t way = tid / kLanes;
+    const uint64_t pitch = (uint64_t)pitch_rows * D;
+    // one row per CTA unless the tile has more than the launch expected
+    for (uint32_t r = r0; row0 + r < row_end; r += tile_rows) {
+        const float2 *ml = part.ml + (uint64_t)r * launched;
+        float m = -INFINITY;
+        for (uint32_t k = tid; k < n; k += kJoinThreads) m = fmaxf(m, ml[k].x);
+        m = all(m, true);
+        const uint32_t row = row0 + r, token = rq.first + row / G, qh = head * G + row % G;
+        for (uint32_t f0 = chunk * 64; f0 < D; f0 += chunks * 64) {
+            const uint32_t f = f0 + tid % kLanes * 4;
+            const float *po = part.o + (uint64_t)r * D + f;
+            float l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t k0 = 0; k0 < n; k0 += kBatch) {
+                const uint32_t count = min(n - k0, kBatch);
+                __syncthreads();
+                for (uint32_t k = tid; k < count; k += kJoinThreads) {
+                    const float2 x = ml[k0 + k];
+                    const float w = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - m);
+                    weight[k] = w;
+                    l += x.y * w;
+                }
+                __syncthreads();
+                for (uint32_t k = way; k < count; k += kWays * kAhead) {
+                    float4 y[kAhead];
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; ++i)
+                        y[i] = k + i * kWays < count ? *reinterpret_cast<const float4 *>(po + (k0 + k + i * kWays) * pitch)
+                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (uint32_t i = 0; i < kAhead; ++i) {
+                        const float w = k + i * kWays < count ? weight[k + i * kWays] : 0.0f;
+                        o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
+                    }
+                }
+            }
+            l = all(l, false);
+            way_sum[way][tid % kLanes] = o;
+            __syncthreads();
+            if (way == 0) {
+#pragma unroll
+                for (uint32_t w = 1; w < kWays; ++w) {
+                    const float4 y = way_sum[w][tid];
+                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                }
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+                if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY))
+                    raise(err, kErrNonFinite);
+                store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
+                if (a.lse != nullptr && f == 0)
+                    a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            }
+        }
     }
 }
 
@@ -915,13 +1040,26 @@ constexpr uint32_t kMaxRowGroups = 128;    // 32 groups to a warp: one batch of 
 constexpr uint32_t kMinRowGroups = 8;
 constexpr uint32_t kMinPromptGroups = 64;
 
+template <int D, int MODE, bool E4M3>
+void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
+                 cudaStream_t stream) {
+    static DeviceOnce once;
+    once.run([] {
+        cudaFuncSetAttribute(kv8_rows_kernel<D, MODE, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kRowSmem<D, terms_of(MODE)>);
+    });
+    KernelTimer timer("kv8_rows", stream);
+    launch_pdl(kv8_rows_kernel<D, MODE, E4M3>, s.requests * h.row_tiles * c.heads * h.row_splits, kRowWarps * 32,
+               kRowSmem<D, terms_of(MODE)>, stream, c, s, a, h, err);
+    count_launch();
+}
+
 template <int D, bool BF16, bool E4M3>
 void launch_all(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
                 cudaStream_t stream) {
     constexpr int TERMS = BF16 ? 1 : 2;
     static DeviceOnce once;
     once.run([] {
-        cudaFuncSetAttribute(kv8_rows_kernel<D, BF16, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem<D, TERMS>);
         cudaFuncSetAttribute(kv8_prompt_kernel<D, BF16, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kPromptSmem<D, TERMS>);
     });
@@ -933,19 +1071,19 @@ void launch_all(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const K
             count_launch();
         }
         if (h.prompt_splits > 1) {
-            launch_pdl(kv8_join_kernel<D, BF16>, h.prompt_tiles * c.heads * (h.prompt_rows / 16), 256, 0, stream, c, s, a, h,
-                       1u, err);
+            launch_pdl(kv8_join_kernel<D, BF16>, h.prompt_tiles * c.heads * h.prompt_rows, kJoinThreads, 0, stream, c, s, a,
+                       h, 1u, err);
             count_launch();
         }
     }
-    {
-        KernelTimer timer("kv8_rows", stream);
-        launch_pdl(kv8_rows_kernel<D, BF16, E4M3>, s.requests * h.row_tiles * c.heads * h.row_splits, kRowWarps * 32,
-                   kRowSmem<D, TERMS>, stream, c, s, a, h, err);
-        count_launch();
-    }
+    if constexpr (BF16)
+        launch_rows<D, kPlain, E4M3>(c, s, a, h, err, stream);
+    else
+        h.row_tile == 8 ? launch_rows<D, kStacked, E4M3>(c, s, a, h, err, stream)
+                        : launch_rows<D, kTwoTerm, E4M3>(c, s, a, h, err, stream);
     if (h.row_splits > 1) {
-        launch_pdl(kv8_join_kernel<D, BF16>, s.requests * h.row_tiles * c.heads, 256, 0, stream, c, s, a, h, 0u, err);
+        launch_pdl(kv8_join_kernel<D, BF16>, s.requests * h.row_tiles * c.heads * h.join_rows * h.join_chunks, kJoinThreads,
+                   0, stream, c, s, a, h, 0u, err);
         count_launch();
     }
 }
@@ -963,7 +1101,8 @@ uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length) {
+Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16,
+                          uint64_t max_kv_length) {
     Kv8Shape h{};
     const uint64_t G = query_heads / c.heads;
     const uint64_t room = (uint64_t)s.columns * c.page_tokens;
@@ -974,12 +1113,15 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
     const bool prompts = rows > kShortRows;
     h.row_tiles = (uint32_t)ceil_div(std::min<uint64_t>(rows, kShortRows), 16);
     h.row_limit = prompts ? kShortRows : UINT32_MAX;
+    h.row_tile = !bf16 && rows <= 8 ? 8 : 16;
     // about two waves of two CTAs per SM if every request were the deepest
     const uint64_t items = (uint64_t)s.requests * h.row_tiles * c.heads;
     uint64_t each = ceil_div(items * groups, 4 * kSms);
     each = std::min<uint64_t>(kMaxRowGroups, std::max<uint64_t>(kMinRowGroups, each));
     h.row_groups = (uint32_t)each;
     h.row_splits = (uint32_t)std::min<uint64_t>(ceil_div(groups, each), 4096);
+    h.join_rows = (uint32_t)std::min<uint64_t>(rows, 16);
+    h.join_chunks = items * h.join_rows < kSms ? c.dim / 64 : 1u;
     h.row_floats = h.row_splits > 1 ? items * h.row_splits * 16 * (c.dim + 2) : 0;
     h.prompt_rows = c.dim == 256 ? kPromptRows<256> : c.dim == 128 ? kPromptRows<128> : kPromptRows<64>;
     if (prompts) {
