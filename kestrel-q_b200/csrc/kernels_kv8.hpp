@@ -50,21 +50,17 @@ struct Kv8Attend {
 
 // How a call's tiles are cut (kv8_attend_shape): by the sizes the host knows.
 struct Kv8Shape {
-    uint32_t row_tile;      // rows per tile of the row kernel: 16, or 8 (F32 only)
-    uint32_t row_tiles;     // its tiles per request
+    uint32_t row_tile;      // rows per tile of the row kernel: 8 or 16
     uint32_t row_limit;     // requests of more rows go to the prompt kernel (UINT32_MAX: none do)
-    uint32_t row_groups;    // 16-token groups per split, row kernel
-    uint32_t row_splits;
-    uint32_t join_rows, join_chunks;   // rows per tile and feature chunks per row that the join is launched for
+    uint32_t row_shares;    // CTAs of the row kernel
+    uint32_t join_wide;     // its cut tiles are joined by a CTA per 64 features of a row
     uint32_t prompt_rows;   // rows per tile of the prompt kernel
     uint32_t prompt_tiles;  // 0: the prompt kernel does not run
     uint32_t prompt_groups, prompt_splits;
     uint64_t row_floats, prompt_floats;   // workspace
 };
 
-// (The work space does not depend on the type.)
-Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16,
-                          uint64_t max_kv_length);
+Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length);
 
 void launch_kv8_plan(const Kv8Cache &c, const Kv8Step &s, const Kv8Plan &p, ErrorWord err, cudaStream_t stream);
 void launch_kv8_append(const Kv8Cache &c, const Kv8Step &s, const void *k, uint64_t k_stride, const void *v,

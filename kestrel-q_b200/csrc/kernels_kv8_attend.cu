@@ -33,16 +33,21 @@
 // loads and no transposes, and a group of 16 tokens is one contiguous bulk
 // copy of 32 * d bytes.
 //
-// Two kernels share the group step:
-//   rows     16 rows per CTA; its four warps take the groups of a split in
-//            turn, each with its own ring of bulk copies and its own softmax
-//            state, and merge at the end.  HBM bound: every (request, head)
-//            reads its codes once.  For single tokens and short chunks.
-//   prompt   8 warps of 16 or 32 rows each share every group of codes; a
-//            ninth warp keeps the ring full.  Bound by the tensor pipe and
-//            the instructions that feed it.
-// Splits of the key axis leave (m, l, O) partials that a third kernel joins
-// in split order, so results do not depend on timing.
+// Two kernels:
+//   rows     8 or 16 query rows per CTA, for single tokens and short chunks.
+//            The rows are the N side of the products (S^T = K Q^T,
+//            O^T = V^T P^T), so that 8 rows waste nothing of an
+//            m16n8k16 and O takes D / 4 registers a thread.  Four warps take
+//            the groups of the CTA's share in turn, each with its own ring of
+//            bulk copies and its own softmax state, and merge at the end.
+//            The launch is cut into equal shares of all (tile, head, group)
+//            units, whatever the requests' lengths; a tile that spans shares
+//            leaves (m, l, O) partials which a second kernel joins in order.
+//            HBM bound: every (request, head) reads its codes once.
+//   prompt   8 warps of 16 or 32 rows each (the M side) share every group of
+//            codes; a ninth warp keeps the ring full.  Bound by the tensor
+//            pipe and the instructions that feed it.
+// Partials are joined in a fixed order: results do not depend on timing.
 #include "kernels_kv8.hpp"
 
 #include <algorithm>
@@ -170,18 +175,8 @@ __device__ __forceinline__ bool load_request(const Kv8Cache &c, const Kv8Step &s
     return ok;
 }
 
-// How a warp's 16 MMA rows are used:
-//   kPlain    16 query rows, fp16-exact queries (bfloat16)
-//   kTwoTerm  16 query rows, every product in two terms (F32)
-//   kStacked  8 query rows: rows 0-7 hold the high parts of Q and of the
-//             weights, rows 8-15 the low parts (F32), so that one product
-//             does both; the halves meet in the same thread's registers
-enum Mode { kPlain, kTwoTerm, kStacked };
-constexpr int terms_of(int mode) { return mode == kTwoTerm ? 2 : 1; }
-constexpr int rows_of(int mode) { return mode == kStacked ? 8 : 16; }
-
 // One tile per warp and MT: softmax state and accumulators.  Thread (g, t) =
-// (lane / 4, lane % 4) holds rows g and, except when stacked, g + 8.
+// (lane / 4, lane % 4) holds rows g and g + 8.
 template <int D, int MT>
 struct Rows {
     float o[MT][D / 8][4];
@@ -206,14 +201,12 @@ struct Rows {
 // [MT][TERMS][D / 16][32 lanes].  factor: per row, softmax scale * log2 e /
 // the row's power of two.  limit: last visible token per row (-1: none);
 // compared only when MASK.
-// The first product's sums run in eight independent accumulators per thread
-// (CH chains per tile): a chain of D / 16 dependent MMAs per group was what
-// the row kernel waited for (302 us against 225 for 64 F32 sequences).
-template <int D, int MT, int NG, int MODE, bool E4M3, bool MASK>
+// The first product's sums run in CH chains where a warp has few tiles: a
+// chain of dependent MMAs waits for each one.
+template <int D, int MT, int NG, int TERMS, bool E4M3, bool MASK>
 __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, const uint8_t *kv, const float (&ks)[NG],
                                            const float (&vs)[NG], const float (&factor)[MT][2],
                                            const int32_t (&limit)[MT][2], int32_t token, uint32_t lane) {
-    constexpr int TERMS = terms_of(MODE), R = MODE == kStacked ? 1 : 2;
     constexpr int CH = MT * NG >= 4 ? 1 : 4 / (MT * NG);
     float s[MT][NG][2][4];
     {
@@ -275,12 +268,12 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
     }
 
     // logits, the rows' maxima
-    float top[MT][R];
+    float top[MT][2];
     bool lift = false;
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int r = 0; r < 2; ++r) {
             float x = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -289,9 +282,7 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float v = s[a][n][h][2 * r + k];
-                        if constexpr (MODE == kStacked) v += s[a][n][h][2 + k];
-                        v *= f;
+                        float v = s[a][n][h][2 * r + k] * f;
                         if (MASK && token + n * 16 + h * 8 + (int32_t)(lane & 3) * 2 + k > limit[a][r]) v = -INFINITY;
                         s[a][n][h][2 * r + k] = v;
                         x = fmaxf(x, v);
@@ -308,13 +299,12 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
         for (int a = 0; a < MT; ++a) {
             float by[2];
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+            for (int r = 0; r < 2; ++r) {
                 const float m = fmaxf(st.m[a][r], top[a][r]);
                 by[r] = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
                 st.m[a][r] = m;
                 st.l[a][r] *= by[r];
             }
-            if constexpr (R == 1) by[1] = by[0];
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -345,31 +335,25 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
     for (int a = 0; a < MT; ++a) {
         float m[2];
 #pragma unroll
-        for (int r = 0; r < R; ++r) m[r] = st.m[a][r] == -INFINITY ? 0.0f : st.m[a][r];
+        for (int r = 0; r < 2; ++r) m[r] = st.m[a][r] == -INFINITY ? 0.0f : st.m[a][r];
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             const float w = vs[n] * inv;
-            float e[2][2 * R];
+            float e[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int k = 0; k < 2 * R; ++k) {
+                for (int k = 0; k < 4; ++k) {
                     e[h][k] = exp2_approx(s[a][n][h][k] - m[k >> 1]);
                     st.l[a][k >> 1] += e[h][k];
                     e[h][k] *= w;
                 }
             }
-            if constexpr (MODE == kStacked) {
-                const uint32_t h0 = pack_half(e[0][0], e[0][1]), h1 = pack_half(e[1][0], e[1][1]);
-                p[a][n][0] = make_uint4(h0, pack_rest(e[0][0], e[0][1], h0), h1, pack_rest(e[1][0], e[1][1], h1));
-            } else {
-                p[a][n][0] = make_uint4(pack_half(e[0][0], e[0][1]), pack_half(e[0][2], e[0][3]),
-                                        pack_half(e[1][0], e[1][1]), pack_half(e[1][2], e[1][3]));
-                if constexpr (TERMS == 2)
-                    p[a][n][1] =
-                        make_uint4(pack_rest(e[0][0], e[0][1], p[a][n][0].x), pack_rest(e[0][2], e[0][3], p[a][n][0].y),
-                                   pack_rest(e[1][0], e[1][1], p[a][n][0].z), pack_rest(e[1][2], e[1][3], p[a][n][0].w));
-            }
+            p[a][n][0] = make_uint4(pack_half(e[0][0], e[0][1]), pack_half(e[0][2], e[0][3]), pack_half(e[1][0], e[1][1]),
+                                    pack_half(e[1][2], e[1][3]));
+            if constexpr (TERMS == 2)
+                p[a][n][1] = make_uint4(pack_rest(e[0][0], e[0][1], p[a][n][0].x), pack_rest(e[0][2], e[0][3], p[a][n][0].y),
+                                        pack_rest(e[1][0], e[1][1], p[a][n][0].z), pack_rest(e[1][2], e[1][3], p[a][n][0].w));
         }
     }
 
@@ -408,61 +392,75 @@ __device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, cons
     }
 }
 
-// Writes rows [row0, row0 + rows_in_tile) of request `rq` as fragments into q
-// and, per row, 1 / its power of two (times the softmax scale in base 2) into
-// factor and its last visible token into limit.  Eight threads per row, every
-// thread of the CTA takes part; rows behind the request's last are zero with
-// limit -1.  Returns whether a query value was not finite.
-template <int D, int MODE, int THREADS, int ROWS>
+// Four query elements from element `at` on.
+template <bool BF16>
+__device__ __forceinline__ float4 load4(const void *base, uint64_t at) {
+    if constexpr (BF16) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(base) + at);
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xffff0000u));
+    } else {
+        return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+    }
+}
+
+// Writes ROWS rows from row0 of request `rq` as fragments into q and, per row,
+// 1 / its power of two (times the softmax scale in base 2) into factor and its
+// last visible token into limit.  Eight threads per row, every thread of the
+// CTA takes part; rows behind the request's last are zero with limit -1.
+// Returns whether a query value was not finite.
+// COLUMNS: the rows are the products' N side, fragments
+// [8-row tile][TERMS][D / 16][32 lanes][2]; else their M side,
+// [16-row tile][TERMS][D / 16][32 lanes][4].
+template <int D, int TERMS, bool COLUMNS, int THREADS, int ROWS>
 __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &rq, uint32_t G, uint32_t head,
-                                             uint32_t row0, uint4 *q, float *factor, int32_t *limit, uint32_t tid) {
-    constexpr int TERMS = terms_of(MODE);
+                                             uint32_t row0, void *q, float *factor, int32_t *limit, uint32_t tid) {
     bool bad = false;
-    uint32_t *q32 = reinterpret_cast<uint32_t *>(q);
+    uint32_t *q32 = static_cast<uint32_t *>(q);
     const uint32_t part = tid & 7;
     for (uint32_t r = tid >> 3; r < ROWS; r += THREADS / 8) {
         const uint32_t row = row0 + r, token = row / G;
         const bool live = token < rq.n;
-        float x[D / 8];
+        float4 x[D / 32];
         float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (live) {
-                const uint64_t at = (uint64_t)(rq.first + token) * a.q_stride + (uint64_t)(head * G + row % G) * D +
-                                    (part + 8 * k) * 4;
-                if constexpr (MODE == kPlain) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(a.q) + at);
-                    v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                                    __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-                } else {
-                    v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
-                }
-            }
-            x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bad |= !(fabsf(x[4 * k + i]) < INFINITY);
-                top = fmaxf(top, fabsf(x[4 * k + i]));
-            }
+            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (live)
+                x[k] = load4<TERMS == 1>(a.q, (uint64_t)(rq.first + token) * a.q_stride + (uint64_t)(head * G + row % G) * D +
+                                                  (part + 8 * k) * 4);
         }
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+            bad |= !(fabsf(x[k].x) < INFINITY) || !(fabsf(x[k].y) < INFINITY) || !(fabsf(x[k].z) < INFINITY) ||
+                   !(fabsf(x[k].w) < INFINITY);
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(x[k].x), fabsf(x[k].y))), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+        }
+        // the eight threads of a row are in one warp; rows run out warp by warp
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
         // the row's largest element into [2^13, 2^14); 2^-100 is the smallest that is still scaled
         const int e = max((int)(__float_as_uint(top) >> 23), 27) - 127 - 13;
         const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
-        const uint32_t tile = r >> 4, half = r >> 3 & 1;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-            const uint32_t f = (part + 8 * k) * 4;
-            const uint32_t at = (((tile * TERMS) * (D / 16) + f / 64 * 4 + f % 16 / 4) * 32 + (r & 7) * 4 + f % 64 / 16) * 4 + half;
-            const uint32_t h0 = pack_half(x[4 * k] * up, x[4 * k + 1] * up), h1 = pack_half(x[4 * k + 2] * up, x[4 * k + 3] * up);
+            const uint32_t f = (part + 8 * k) * 4, step = f / 64 * 4 + f % 16 / 4, lane = (r & 7) * 4 + f % 64 / 16;
+            const float a0 = x[k].x * up, a1 = x[k].y * up, a2 = x[k].z * up, a3 = x[k].w * up;
+            const uint32_t h0 = pack_half(a0, a1), h1 = pack_half(a2, a3);
+            // places of the pair (features f, f + 1), of the next pair and of the low terms
+            uint32_t at, next, low;
+            if constexpr (COLUMNS) {
+                at = (((r >> 3) * TERMS * (D / 16) + step) * 32 + lane) * 2;
+                next = 1, low = D / 16 * 64;
+            } else {
+                at = (((r >> 4) * TERMS * (D / 16) + step) * 32 + lane) * 4 + (r >> 3 & 1);
+                next = 2, low = D / 16 * 128;
+            }
             q32[at] = h0;
-            q32[at + 2] = h1;
-            if constexpr (MODE != kPlain) {
-                constexpr uint32_t low = MODE == kStacked ? 1 : D / 16 * 128;   // rows 8-15, or the second term
-                q32[at + low] = pack_rest(x[4 * k] * up, x[4 * k + 1] * up, h0);
-                q32[at + low + 2] = pack_rest(x[4 * k + 2] * up, x[4 * k + 3] * up, h1);
+            q32[at + next] = h1;
+            if constexpr (TERMS == 2) {
+                q32[at + low] = pack_rest(a0, a1, h0);
+                q32[at + low + next] = pack_rest(a2, a3, h1);
             }
         }
         if (part == 0) {
@@ -483,6 +481,20 @@ __device__ __forceinline__ void store4(void *out, uint64_t at, float4 v) {
     } else {
         *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = v;
     }
+}
+
+// Four features of a row from its sums: the output and, with the first four,
+// the log-sum.
+template <bool BF16>
+__device__ __forceinline__ void finish4(const Kv8Attend &a, const Request &rq, uint32_t G, uint32_t head, uint32_t row,
+                                        uint32_t f, uint32_t dim, float m, float l, float4 o, const ErrorWord &err) {
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY)) raise(err, kErrNonFinite);
+    const uint64_t token = rq.first + row / G;
+    const uint32_t qh = head * G + row % G;
+    store4<BF16>(a.out, token * a.out_stride + (uint64_t)qh * dim + f, o);
+    if (a.lse != nullptr && f == 0) a.lse[token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // Where the partials of a (tile, head) lie: O [split][row][D], and behind the
@@ -510,71 +522,302 @@ __device__ __forceinline__ uint32_t split_groups(uint32_t groups, uint32_t each,
     return max(each, ((groups + splits - 1) / splits + unit - 1) / unit * unit);
 }
 
-template <int D> constexpr int kRowStages = D == 256 ? 3 : 6;
-constexpr int kRowWarps = 4;
-template <int D, int TERMS> constexpr uint32_t kRowSmem = kRowWarps * kRowStages<D> * 32 * D + TERMS * 32 * D;
+// ------------------------------------------------------------------- rows
+
+constexpr int kRowWarps = 4, kRowThreads = kRowWarps * 32;
+constexpr uint32_t kMinShare = 2 * kRowWarps;   // units: two groups to a warp
+// CTAs per SM and ring slots per warp: registers hold NT * D / 4 accumulators
+// a thread, shared memory the rings (and, at the end, the warps' merge).
+template <int D, int NT> constexpr int kRowCtas = NT * D == 512 ? 2 : D == 256 || NT * D == 256 ? 3 : 4;
+template <int D, int NT> constexpr int kRowStages = NT * D == 512 ? 3 : D == 256 ? 2 : NT * D == 256 ? 4 : D == 128 ? 3 : 5;
+template <int D, int NT, int TERMS>
+constexpr uint32_t kRowSmem = kRowWarps * kRowStages<D, NT> * 32 * D + NT * TERMS * 16 * D;
+
+// A warp's softmax state and accumulators of NT tiles of 8 rows.  Thread (g, t)
+// = (lane / 4, lane % 4) holds rows 2t and 2t + 1 of each tile.
+template <int D, int NT>
+struct Columns {
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2], ref;
+
+    __device__ __forceinline__ void clear() {
+        ref = 0.0f;
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) m[a][r] = -INFINITY, l[a][r] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[a][n][k] = 0.0f;
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// One step over a group of 16 tokens with the rows on the N side.  A key
+// fragment's rows are tokens g and g + 8; a value fragment's rows are features
+// 4 g + i and 4 g + i + 1 of 32.  The weights come out of the first product
+// with tokens as rows and are turned by movmatrix.  The first product runs in
+// four chains of MMAs (one chain per group was what this kernel waited for).
+template <int D, int NT, int TERMS, bool E4M3, bool MASK>
+__device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, const uint8_t *kv, float ks, float vs,
+                                            const float (&factor)[NT][2], const int32_t (&limit)[NT][2], int32_t token,
+                                            uint32_t lane) {
+    constexpr int CH = 4 / NT;
+    float c[CH][NT][4];
+#pragma unroll
+    for (int x = 0; x < CH; ++x)
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) c[x][a][k] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        const uint4 w0 = *reinterpret_cast<const uint4 *>(kv + j * 1024 + lane * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4 *>(kv + j * 1024 + 512 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint4 x;
+            widen<E4M3>(i == 0 ? w0.x : i == 1 ? w0.y : i == 2 ? w0.z : w0.w, x.x, x.z);
+            widen<E4M3>(i == 0 ? w1.x : i == 1 ? w1.y : i == 2 ? w1.z : w1.w, x.y, x.w);
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                    const uint2 f = q[((a * TERMS + term) * (D / 16) + j * 4 + i) * 32 + lane];
+                    mma(c[(i * TERMS + term) % CH][a], x, f.x, f.y);
+                }
+        }
+    }
+    float s[NT][4], top[NT][2];
+    bool lift = false;
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v = c[0][a][k];
+#pragma unroll
+            for (int x = 1; x < CH; ++x) v += c[x][a][k];
+            v *= factor[a][k & 1] * ks;
+            if (MASK && token + (k >> 1) * 8 + (int32_t)(lane >> 2) > limit[a][k & 1]) v = -INFINITY;
+            s[a][k] = v;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float x = fmaxf(s[a][r], s[a][2 + r]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+            top[a][r] = x;
+            lift |= x > st.m[a][r] + kRaise;
+        }
+    }
+    if (__any_sync(~0u, lift)) {   // -inf + 8 is -inf: the first finite logit of a row lifts it
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            float by[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float m = fmaxf(st.m[a][r], top[a][r]);
+                by[r] = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
+                st.m[a][r] = m;
+                st.l[a][r] *= by[r];
+            }
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by[k & 1];
+        }
+    }
+    if (vs > st.ref) {
+        // the next power of two, within the normal range
+        const uint32_t e = min((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
+        const float ref = __uint_as_float(max(e, 0x00800000u));
+        const float by = st.ref / ref;
+        st.ref = ref;
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by;
+    }
+    const float w = st.ref > 0.0f ? vs * (kWeightScale / st.ref) : 0.0f;
+    uint2 p[NT][TERMS];
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            e[k] = exp2_approx(s[a][k] - (st.m[a][k & 1] == -INFINITY ? 0.0f : st.m[a][k & 1]));
+            st.l[a][k & 1] += e[k];
+            e[k] *= w;
+        }
+        const uint32_t h0 = pack_half(e[0], e[1]), h1 = pack_half(e[2], e[3]);
+        p[a][0] = make_uint2(transpose8x8(h0), transpose8x8(h1));
+        if constexpr (TERMS == 2)
+            p[a][1] = make_uint2(transpose8x8(pack_rest(e[0], e[1], h0)), transpose8x8(pack_rest(e[2], e[3], h1)));
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(kv + 16 * D + j * 512 + lane * 16);
+        uint4 x[2];
+        widen<E4M3>(v.x, x[0].x, x[0].z);
+        widen<E4M3>(v.y, x[0].y, x[0].w);
+        widen<E4M3>(v.z, x[1].x, x[1].z);
+        widen<E4M3>(v.w, x[1].y, x[1].w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+                for (int term = TERMS - 1; term >= 0; --term) mma(st.o[a][j * 2 + i], x[i], p[a][term].x, p[a][term].y);
+    }
+}
+
+// The row kernel's share of the work.  A unit is one group of one (request,
+// tile, head); every tile of a request counts as many as its last one sees.
+// The launch's shares are as many as the sizes the host knows can use; of
+// these the first `total / kMinShare` work, so that none is empty or tiny.
+// The first unit of share k of n over `total` units:
+__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t k, uint32_t n) { return total * k / n; }
+
+__device__ __forceinline__ uint32_t row_items(const Request &rq, uint32_t G, uint32_t tile_rows, uint32_t heads,
+                                              uint64_t row_limit) {
+    const uint64_t rows = (uint64_t)rq.n * G;
+    return rows > row_limit ? 0u : (uint32_t)((rows + tile_rows - 1) / tile_rows) * heads;
+}
+
+// At least one, so that a request without cached tokens still gets its zeros.
+__device__ __forceinline__ uint32_t item_units(const Request &rq) { return max(1u, (rq.length + kG - 1) / kG); }
+
+// What share k leaves for the join: the tile that it begins and does not end.
+struct Cut {
+    uint32_t request, tile, head, last;   // last: the share that ends it (0: nothing was cut)
+};
+
+// A share's partials: [share][ended, begun] of [rows][D] floats, then (m, l)
+// per row, then the cuts.
+struct ShareSpace {
+    float *o;
+    float2 *ml;
+    Cut *cuts;
+    __device__ __forceinline__ ShareSpace(float *base, uint32_t shares, uint32_t rows, uint32_t dim) {
+        o = base;
+        ml = reinterpret_cast<float2 *>(base + 2ull * shares * rows * dim);
+        cuts = reinterpret_cast<Cut *>(ml + 2ull * shares * rows);
+    }
+};
 
 }  // namespace
 
-// grid (request, tile, head, split); four warps, 16 or 8 rows.  Each warp streams
-// every fourth group of the split through its own ring; page ids and scales of
-// a warp's next 32 groups sit in its lanes.
-// Partials: [request][tile][head][split][16 rows][D], then (m, l) per row.
-template <int D, int MODE, bool E4M3>
-__global__ void __launch_bounds__(kRowWarps * 32, 2)
+// grid: equal shares of all units.  Each warp streams every fourth group of a
+// tile through its own ring; page ids and scales of its next 64 groups sit in
+// its lanes.
+// Measured: see the launch rules below (kv8_attend_shape).
+template <int D, int NT, int TERMS, bool E4M3>
+__global__ void __launch_bounds__(kRowThreads, (kRowCtas<D, NT>))
 kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr int ST = kRowStages<D>;
-    constexpr bool BF16 = MODE == kPlain;
-    constexpr uint32_t kStage = 32 * D, kRows = rows_of(MODE), kR = MODE == kStacked ? 1 : 2;
+    constexpr int ST = kRowStages<D, NT>;
+    constexpr bool BF16 = TERMS == 1;
+    constexpr uint32_t kStage = 32 * D, kRows = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kRowWarps][ST];
-    __shared__ float factor_s[16], merge_m[kRowWarps][16], merge_l[kRowWarps][16];
-    __shared__ int32_t limit_s[16];
+    __shared__ float factor_s[kRows], merge_m[kRowWarps][kRows], merge_l[kRowWarps][kRows];
+    __shared__ int32_t limit_s[kRows];
+    __shared__ uint64_t warp_units[kRowWarps], begin_unit;
+    __shared__ uint32_t begin_request;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint8_t *ring = smem + warp * ST * kStage;
-    uint4 *q = reinterpret_cast<uint4 *>(smem + kRowWarps * ST * kStage);
-    const uint32_t G = a.query_heads / c.heads;
-    const uint32_t split = blockIdx.x % shape.row_splits, u = blockIdx.x / shape.row_splits;
-    const uint32_t head = u % c.heads, tile0 = u / c.heads % shape.row_tiles, b = u / c.heads / shape.row_tiles;
+    uint2 *q = reinterpret_cast<uint2 *>(smem + kRowWarps * ST * kStage);
+    const uint32_t G = a.query_heads / c.heads, share = blockIdx.x, shares = gridDim.x;
+    const ShareSpace space(a.workspace, shares, kRows, D);
 
     if (tid < kRowWarps * ST) bar_init(&full[0][0] + tid, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pdl_wait();
     if (__syncthreads_or(tid == 0 && err_raised(err))) return;
-    Request rq;
-    if (!load_request(c, s, b, rq, err)) return;
-    const uint64_t rows64 = (uint64_t)rq.n * G;
-    if (rows64 == 0 || rows64 > shape.row_limit) return;
-    const uint32_t rows = (uint32_t)rows64;
-    // a request of more tiles than the launch has is not split: its partials
-    // would have no place
-    const uint32_t splits = (rows + kRows - 1) / kRows > shape.row_tiles ? 1u : shape.row_splits;
-    const int32_t *table = s.table + (uint64_t)b * s.table_stride;
-    const uint32_t per_page = c.page_tokens / kG;
-    const uint64_t page_bytes = 2ull * c.page_tokens * D;
-    uint32_t used = 0;   // ring slots used so far (waits go by it)
 
-    for (uint32_t tile = tile0; tile * kRows < rows; tile += shape.row_tiles) {
-        const uint32_t row0 = tile * kRows, row_end = min(row0 + kRows, rows);
-        const uint32_t groups = visible_groups(rq, G, row_end), each = split_groups(groups, shape.row_groups, splits, 1);
-        const uint32_t g0 = split * each, g1 = min(g0 + each, groups);
-        if (split > 0 && g0 >= groups) break;   // later tiles see more groups only when splits == 1
+    // units of all requests: consecutive requests per thread, then the request
+    // in which this share begins
+    Request rq;
+    const uint32_t per = (s.requests + kRowThreads - 1) / kRowThreads;
+    const uint32_t b0 = min(tid * per, s.requests), b1 = min(b0 + per, s.requests);
+    uint64_t units = 0;
+    bool good = true;
+    for (uint32_t b = b0; b < b1; ++b)
+        if (load_request(c, s, b, rq, err))
+            units += (uint64_t)row_items(rq, G, kRows, c.heads, shape.row_limit) * item_units(rq);
+        else
+            good = false;
+    uint64_t upto = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= (uint32_t)o) upto += x;
+    }
+    if (lane == 31) warp_units[warp] = upto;
+    if (__syncthreads_or(!good)) return;
+    uint64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+        if (w < (int)warp) upto += warp_units[w];
+        total += warp_units[w];
+    }
+    if (shares > 1 && tid == 0) space.cuts[share].last = 0;
+    const uint32_t working = (uint32_t)min((uint64_t)shares, max(total / kMinShare, (uint64_t)1));
+    if (share >= working || total == 0) return;
+    uint64_t at = share_begin(total, share, working);
+    const uint64_t end = share_begin(total, share + 1, working);
+    if (at >= upto - units && at < upto) {
+        uint64_t left = at - (upto - units);
+        for (uint32_t b = b0; b < b1; ++b) {
+            load_request(c, s, b, rq, err);
+            const uint64_t n = (uint64_t)row_items(rq, G, kRows, c.heads, shape.row_limit) * item_units(rq);
+            if (left < n) {
+                begin_request = b;
+                begin_unit = left;
+                break;
+            }
+            left -= n;
+        }
+    }
+    __syncthreads();
+    uint32_t b = begin_request;
+    uint64_t inside = begin_unit;   // unit of request b
+    load_request(c, s, b, rq, err);
+
+    uint32_t used = 0;   // ring slots used so far (waits go by it)
+    while (true) {
+        const uint32_t depth = item_units(rq), item = (uint32_t)(inside / depth), u0 = (uint32_t)(inside % depth);
+        const uint32_t tile = item / c.heads, head = item % c.heads;
+        const uint32_t u1 = (uint32_t)min((uint64_t)depth, u0 + (end - at));
+        const uint32_t rows = rq.n * G, row0 = tile * kRows, row_end = min(row0 + kRows, rows);
+        const uint32_t groups = visible_groups(rq, G, row_end), g0 = min(u0, groups), g1 = min(u1, groups);
+        const int32_t *table = s.table + (uint64_t)b * s.table_stride;
+        const uint32_t per_page = c.page_tokens / kG;
+        const uint64_t page_bytes = 2ull * c.page_tokens * D;
         // this warp's groups: g0 + warp + 4 i
         const uint32_t mine = g1 > g0 + warp ? (g1 - g0 - warp + kRowWarps - 1) / kRowWarps : 0;
-        uint32_t page = 0;
-        float2 scales = make_float2(0.0f, 0.0f);
-        auto fetch = [&](uint32_t from) {   // page ids and scales of groups from .. from + 31
+        uint32_t page[2] = {0, 0};   // page ids and scales of 32 groups, and of the next 32
+        float2 scales[2] = {};
+        auto fetch = [&](uint32_t from, int k) {
             const uint32_t i = from + lane;
             if (i < mine) {
                 const int32_t id = table[(g0 + warp + i * kRowWarps) / per_page];
                 const bool ok = id >= 0 && (uint32_t)id < c.pages;
                 if (!ok) raise(err, kErrStep);
-                page = ok ? (uint32_t)id : 0u;   // any page: the call fails
-                scales = *reinterpret_cast<const float2 *>(c.scales + ((uint64_t)page * c.heads + head) * 2);
+                page[k] = ok ? (uint32_t)id : 0u;   // any page: the call fails
+                scales[k] = *reinterpret_cast<const float2 *>(c.scales + ((uint64_t)page[k] * c.heads + head) * 2);
             }
         };
-        auto issue = [&](uint32_t i) {   // group i of this warp into its slot; page ids are in the lanes
-            const uint32_t id = __shfl_sync(~0u, page, i & 31);
+        auto issue = [&](uint32_t i, uint32_t from) {   // group i of this warp into its slot; lanes hold from .. from + 63
+            const uint32_t id = __shfl_sync(~0u, i - from < 32 ? page[0] : page[1], i & 31);
             if (lane == 0) {
                 const uint32_t slot = (used + i) % ST;
                 bar_expect(&full[warp][slot], kStage);
@@ -584,40 +827,47 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
                           kStage, &full[warp][slot]);
             }
         };
-        fetch(0);
+        fetch(0, 0);
         uint32_t issued = 0;
-        for (; issued < min(mine, (uint32_t)ST); ++issued) issue(issued);
+        for (; issued < min(mine, (uint32_t)ST); ++issued) issue(issued, 0);
+        fetch(32, 1);
 
-        if (load_queries<D, MODE, kRowWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
+        if (load_queries<D, TERMS, true, kRowThreads, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
             raise(err, kErrNonFinite);
         __syncthreads();
-        Rows<D, 1> st;
+        Columns<D, NT> st;
         st.clear();
-        const float factor[1][2] = {{factor_s[lane >> 2], factor_s[(lane >> 2) + 8 * (kR - 1)]}};
-        const int32_t limit[1][2] = {{limit_s[lane >> 2], limit_s[(lane >> 2) + 8 * (kR - 1)]}};
-        // every row of the tile sees the tokens up to its first token's
-        const uint32_t clear_to = rq.length + 1 > rq.n ? rq.length - rq.n + row0 / G + 1 : 0u;
+        float factor[NT][2];
+        int32_t limit[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                factor[n][r] = factor_s[n * 8 + (lane & 3) * 2 + r];
+                limit[n][r] = limit_s[n * 8 + (lane & 3) * 2 + r];
+            }
+        // every row of the tile sees the tokens before this one
+        const uint32_t clear_to = row_end == row0 + kRows && rq.length + 1 > rq.n ? rq.length - rq.n + row0 / G + 1 : 0u;
         bool ok = true;
         uint32_t i = 0;
-        for (; i < mine && ok; ++i) {
+        for (; i < mine; ++i) {
             if (i > 0 && (i & 31) == 0) {
-                // the lanes' next 32 groups; the ring runs dry here once per 128 groups of the split
-                fetch(i);
-                for (; issued < min(mine, i + ST); ++issued) issue(issued);
+                page[0] = page[1];
+                scales[0] = scales[1];
+                fetch(i + 32, 1);
             }
             const uint32_t slot = (used + i) % ST;
             ok = bar_wait(&full[warp][slot], (used + i) / ST & 1u);
             if (!ok) break;
-            const float ks[1] = {__shfl_sync(~0u, scales.x, i & 31)}, vs[1] = {__shfl_sync(~0u, scales.y, i & 31)};
+            const float ks = __shfl_sync(~0u, scales[0].x, i & 31), vs = __shfl_sync(~0u, scales[0].y, i & 31);
             const uint32_t token = (g0 + warp + i * kRowWarps) * kG;
             const uint8_t *kv = ring + slot * kStage;
-            if (token + kG > clear_to || row_end < row0 + kRows)
-                group_step<D, 1, 1, MODE, E4M3, true>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
+            if (token + kG > clear_to)
+                column_step<D, NT, TERMS, E4M3, true>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
             else
-                group_step<D, 1, 1, MODE, E4M3, false>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                column_step<D, NT, TERMS, E4M3, false>(st, q, kv, ks, vs, factor, limit, (int32_t)token, lane);
             __syncwarp();
-            // refill only with groups whose page ids the lanes hold
-            if (issued < mine && (issued & ~31u) == (i & ~31u)) issue(issued++);
+            if (issued < mine) issue(issued++, i & ~31u);
         }
         if (!ok) {
             // a wait gave up: let the other copies land before the CTA exits
@@ -628,41 +878,33 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
 
         // join the warps: (m, l) and O of each in its own ring
 #pragma unroll
-        for (int r = 0; r < (int)kR; ++r) {
-            st.l[0][r] += __shfl_xor_sync(~0u, st.l[0][r], 1);
-            st.l[0][r] += __shfl_xor_sync(~0u, st.l[0][r], 2);
-        }
-        if ((lane & 3) == 0) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < (int)kR; ++r) {
-                merge_m[warp][(lane >> 2) + 8 * r] = st.m[0][r];
-                merge_l[warp][(lane >> 2) + 8 * r] = st.l[0][r];
+            for (int r = 0; r < 2; ++r) {
+                float l = st.l[n][r];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(~0u, l, o);
+                if (lane < 4) {
+                    merge_m[warp][n * 8 + lane * 2 + r] = st.m[n][r];
+                    merge_l[warp][n * 8 + lane * 2 + r] = l;
+                }
             }
-        }
         constexpr uint32_t kPitch = D + 4;   // rows 4 banks apart: conflict-free 16-byte stores
         float *mo = reinterpret_cast<float *>(ring);
         const float back = st.ref * (1.0f / kWeightScale);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < (int)kR; ++r)
+            for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = st.o[0][4 * j + i][2 * r + k];
-                        if constexpr (MODE == kStacked) x[i] += st.o[0][4 * j + i][2 + k];
-                        x[i] *= back;
-                    }
-                    *reinterpret_cast<float4 *>(mo + ((lane >> 2) + 8 * r) * kPitch + j * 32 + (lane & 3) * 8 + 4 * k) =
-                        make_float4(x[0], x[1], x[2], x[3]);
-                }
+                for (int r = 0; r < 2; ++r)
+                    *reinterpret_cast<float4 *>(mo + (n * 8 + (lane & 3) * 2 + r) * kPitch + j * 32 + (lane >> 2) * 4) =
+                        make_float4(st.o[n][2 * j][r] * back, st.o[n][2 * j][2 + r] * back, st.o[n][2 * j + 1][r] * back,
+                                    st.o[n][2 * j + 1][2 + r] * back);
         __syncthreads();
-        const bool whole = groups <= each;   // one split: the result itself
-        const Partials part(a.workspace, ((uint64_t)b * shape.row_tiles + tile) * c.heads + head, shape.row_splits, 16, D,
-                            (uint64_t)s.requests * shape.row_tiles * c.heads);
-        for (uint32_t v = tid; v < (row_end - row0) * (D / 4); v += kRowWarps * 32) {
+        const bool begun = u0 == 0, ended = u1 == depth;
+        const uint64_t place = 2ull * share + (begun ? 1 : 0);   // of a partial
+        for (uint32_t v = tid; v < (row_end - row0) * (D / 4); v += kRowThreads) {
             const uint32_t r = v / (D / 4), f = v % (D / 4) * 4;
             float m = merge_m[0][r];
 #pragma unroll
@@ -677,24 +919,113 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
                 l += merge_l[w][r] * by;
                 o.x += x.x * by, o.y += x.y * by, o.z += x.z * by, o.w += x.w * by;
             }
-            if (whole) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-                if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY))
-                    raise(err, kErrNonFinite);
-                const uint32_t row = row0 + r, token = rq.first + row / G, qh = head * G + row % G;
-                store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
-                if (a.lse != nullptr && f == 0)
-                    a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            if (begun && ended) {
+                finish4<BF16>(a, rq, G, head, row0 + r, f, D, m, l, o, err);
             } else {
-                *reinterpret_cast<float4 *>(part.o + ((uint64_t)split * 16 + r) * D + f) = o;
-                if (f == 0) part.ml[r * shape.row_splits + split] = make_float2(m, l);
+                *reinterpret_cast<float4 *>(space.o + (place * kRows + r) * D + f) = o;
+                if (f == 0) space.ml[place * kRows + r] = make_float2(m, l);
             }
         }
-        if (__syncthreads_or(!ok)) return;
-        // the ring, the queries and the merge are free again; the ring's next
-        // writes come through the asynchronous proxy
+        if (begun && !ended && tid == 0)
+            space.cuts[share] = {b, tile, head, (uint32_t)(((at + (depth - u0)) * working - 1) / total)};
+        // the ring's next writes come through the asynchronous proxy
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (__syncthreads_or(!ok)) return;
+        at += u1 - u0;
+        if (at >= end) return;
+        inside += u1 - u0;
+        // the next request that has units (there is one: at < end)
+        while (inside >= (uint64_t)row_items(rq, G, kRows, c.heads, shape.row_limit) * depth || rq.n == 0) {
+            inside = 0;
+            if (++b >= s.requests) return;
+            load_request(c, s, b, rq, err);
+            if (row_items(rq, G, kRows, c.heads, shape.row_limit) > 0) break;
+            rq.n = 0;
+        }
+    }
+}
+
+namespace {
+
+constexpr int kShareJoinThreads = 256;
+
+}  // namespace
+
+// Joins the tiles that shares cut: CTA (share k, chunk) takes the tile that
+// share k began, from shares k .. last in this order.  A chunk is 64 features
+// of one row, its partials dealt to 16 groups of 16 threads (WIDE, for a few
+// tiles of many partials), or all of the tile with a thread per 4 features.
+// Bound: latency, the partials come from L2.
+template <int D, int NT, bool BF16, bool WIDE>
+__global__ void __launch_bounds__(kShareJoinThreads)
+kv8_rows_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
+    constexpr uint32_t kRows = 8 * NT, kCells = kRows * (D / 4);
+    constexpr uint32_t kChunks = WIDE ? kRows * (D / 64) : 1, kWays = WIDE ? 16 : 1, kAhead = 8;
+    __shared__ float4 way_o[kWays][WIDE ? 16 : 1];
+    __shared__ float way_m[kWays], way_l[kWays];
+    const uint32_t tid = threadIdx.x, share = blockIdx.x / kChunks, chunk = blockIdx.x % kChunks;
+    const uint32_t G = a.query_heads / c.heads;
+    pdl_wait();
+    if (__syncthreads_or(tid == 0 && err_raised(err))) return;
+    const ShareSpace space(a.workspace, shape.row_shares, kRows, D);
+    const Cut cut = space.cuts[share];
+    if (cut.last <= share) return;
+    Request rq;
+    if (!load_request(c, s, cut.request, rq, err)) return;
+    const uint32_t row0 = cut.tile * kRows, row_end = min(row0 + kRows, rq.n * G), n = cut.last - share + 1;
+    const uint32_t way = WIDE ? tid / 16 : 0u;
+    for (uint32_t v = WIDE ? chunk * 16 + tid % 16 : tid; v < kCells; v += WIDE ? kCells : kShareJoinThreads) {
+        const uint32_t r = v / (D / 4), f = v % (D / 4) * 4;
+        if (row0 + r >= row_end) break;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t k = way; k < n; k += kWays * kAhead) {
+            float4 y[kAhead];
+            float2 x[kAhead];
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const uint32_t at = k + i * kWays;
+                // the first share's partial is the one it began, the others' the one they ended or passed through
+                const uint64_t place = 2ull * (share + at) + (at == 0 ? 1 : 0);
+                const bool in = at < n;
+                y[i] = in ? *reinterpret_cast<const float4 *>(space.o + (place * kRows + r) * D + f)
+                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                x[i] = in ? space.ml[place * kRows + r] : make_float2(-INFINITY, 0.0f);
+            }
+            float top = m;
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].x);
+            if (top == -INFINITY) continue;
+            const float by = exp2_approx(m - top);
+            m = top;
+            l *= by, o.x *= by, o.y *= by, o.z *= by, o.w *= by;
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const float w = exp2_approx(x[i].x - m);
+                l += x[i].y * w;
+                o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
+            }
+        }
+        if constexpr (WIDE) {
+            way_o[way][tid % 16] = o;
+            if (tid % 16 == 0) way_m[way] = m, way_l[way] = l;
+            __syncthreads();   // all threads of the CTA are on the same row
+            if (way > 0) return;
+            float top = way_m[0];
+#pragma unroll
+            for (uint32_t w = 1; w < kWays; ++w) top = fmaxf(top, way_m[w]);
+            l = 0.0f;
+            o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t w = 0; w < kWays; ++w) {
+                const float by = way_m[w] == -INFINITY ? 0.0f : exp2_approx(way_m[w] - top);
+                const float4 y = way_o[w][tid % 16];
+                l += way_l[w] * by;
+                o.x += y.x * by, o.y += y.y * by, o.z += y.z * by, o.w += y.w * by;
+            }
+            m = top;
+        }
+        finish4<BF16>(a, rq, G, cut.head, row0 + r, f, D, m, l, o, err);
     }
 }
 
@@ -743,7 +1074,7 @@ __device__ __forceinline__ uint32_t find_request(const Kv8Step &s, uint32_t G, u
 template <int D, bool BF16, bool E4M3>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr int MODE = BF16 ? kPlain : kTwoTerm, TERMS = terms_of(MODE), MT = kPromptMt<D>, ST = kPromptStages<D>, NG = kPromptGroups;
+    constexpr int TERMS = BF16 ? 1 : 2, MT = kPromptMt<D>, ST = kPromptStages<D>, NG = kPromptGroups;
     constexpr uint32_t kGroup = 32 * D, kStage = NG * kGroup, kRows = kPromptRows<D>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[ST], empty[ST];
@@ -821,7 +1152,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
 
-    if (load_queries<D, MODE, kPromptWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
+    if (load_queries<D, TERMS, false, kPromptWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
         raise(err, kErrNonFinite);
     asm volatile("bar.sync 1, %0;" ::"n"(kPromptWarps * 32) : "memory");
     Rows<D, MT> st;
@@ -854,9 +1185,9 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             const float ks[NG] = {s0.x, s1.x}, vs[NG] = {s0.y, s1.y};
             const uint8_t *kv = smem + slot * kStage;
             if (token + NG * kG > all_see || g0 + (k + 1) * NG > g1)
-                group_step<D, MT, NG, MODE, E4M3, true>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                group_step<D, MT, NG, TERMS, E4M3, true>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
             else
-                group_step<D, MT, NG, MODE, E4M3, false>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
+                group_step<D, MT, NG, TERMS, E4M3, false>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
         }
         __syncwarp();
         if (lane == 0) bar_arrive(&empty[slot]);
@@ -912,121 +1243,52 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
 
 constexpr int kJoinThreads = 256;
 
-// Joins the splits of a row: one CTA per (tile, head, row), or per 64 features
-// of it where there are few.  The threads first turn the splits' (m, l) into
-// weights 2^(m_k - m) in shared memory, 1024 at a time; 16 threads then hold 4
-// features each of every 16th split, and meet in shared memory in a fixed
-// order.  Bound: latency, the partials come from L2.
+// Joins the splits of a prompt tile: one CTA per (tile, head, 16 rows), a
+// thread per 4 features of a row, in split order.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads)
-kv8_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, uint32_t prompt, ErrorWord err) {
-    constexpr uint32_t kLanes = 16, kWays = kJoinThreads / kLanes, kBatch = 1024, kAhead = 8;
-    __shared__ float weight[kBatch];
-    __shared__ float warp_red[kJoinThreads / 32];
-    __shared__ float4 way_sum[kWays][kLanes];
-    const uint32_t tid = threadIdx.x, lane = tid & 31, G = a.query_heads / c.heads;
-    const uint32_t tile_rows = prompt ? shape.prompt_rows : shape.join_rows;
-    const uint32_t chunks = prompt ? 1u : shape.join_chunks;
-    const uint32_t chunk = blockIdx.x % chunks, r0 = blockIdx.x / chunks % tile_rows;
-    const uint32_t u = blockIdx.x / chunks / tile_rows, head = u % c.heads, slot = u / c.heads;
+kv8_prompt_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
+    constexpr uint32_t kRows = kPromptRows<D>, kAhead = 8;
+    const uint32_t tid = threadIdx.x, G = a.query_heads / c.heads;
+    const uint32_t block = blockIdx.x % (kRows / 16), u = blockIdx.x / (kRows / 16), head = u % c.heads, t = u / c.heads;
     pdl_wait();
     if (__syncthreads_or(tid == 0 && err_raised(err))) return;
-    uint32_t b, tile;
-    if (prompt) {
-        uint32_t start;
-        b = find_request(s, G, tile_rows, slot, lane, start);
-        if (slot < start) return;
-        tile = slot - start;
-    } else {
-        b = slot / shape.row_tiles;
-        tile = slot % shape.row_tiles;
-    }
+    uint32_t start;
+    const uint32_t b = find_request(s, G, kRows, t, tid & 31, start);
     Request rq;
-    if (!load_request(c, s, b, rq, err)) return;
+    if (t < start || !load_request(c, s, b, rq, err)) return;
     const uint64_t rows64 = (uint64_t)rq.n * G;
-    const uint32_t held = prompt ? shape.prompt_rows : shape.row_tile, pitch_rows = prompt ? shape.prompt_rows : 16u;
-    if (prompt ? rows64 <= shape.row_limit : rows64 > shape.row_limit) return;
-    if (!prompt && (rows64 + held - 1) / held > shape.row_tiles) return;
-    if ((uint64_t)tile * held >= rows64) return;
-    const uint32_t rows = (uint32_t)rows64, row0 = tile * held, row_end = min(row0 + held, rows);
-    const uint32_t launched = prompt ? shape.prompt_splits : shape.row_splits;
+    if (rows64 <= shape.row_limit || (uint64_t)(t - start) * kRows >= rows64) return;
+    const uint32_t rows = (uint32_t)rows64, row0 = (t - start) * kRows, row_end = min(row0 + kRows, rows);
     const uint32_t groups = visible_groups(rq, G, row_end);
-    const uint32_t each = split_groups(groups, prompt ? shape.prompt_groups : shape.row_groups, launched,
-                                       prompt ? kPromptGroups : 1u);
+    const uint32_t each = split_groups(groups, shape.prompt_groups, shape.prompt_splits, kPromptGroups);
     if (groups <= each) return;
     const uint32_t n = (groups + each - 1) / each;
-    const Partials part(a.workspace + (prompt ? shape.row_floats : 0), (uint64_t)slot * c.heads + head, launched, pitch_rows,
-                        D, (uint64_t)(prompt ? shape.prompt_tiles : s.requests * shape.row_tiles) * c.heads);
-
-    auto all = [&](float v, bool take_max) {   // over the CTA, the same in every thread
+    const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, kRows, D,
+                        (uint64_t)shape.prompt_tiles * c.heads);
+    for (uint32_t v = tid; v < 16 * (D / 4); v += kJoinThreads) {
+        const uint32_t r = block * 16 + v / (D / 4), f = v % (D / 4) * 4;
+        if (row0 + r >= row_end) break;
+        const float2 *ml = part.ml + (uint64_t)r * shape.prompt_splits;
+        const float *po = part.o + (uint64_t)r * D + f;
+        float m = -INFINITY, l = 0.0f;
+        for (uint32_t k = 0; k < n; ++k) m = fmaxf(m, ml[k].x);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t k = 0; k < n; k += kAhead) {
+            float4 y[kAhead];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float x = __shfl_xor_sync(~0u, v, o);
-            v = take_max ? fmaxf(v, x) : v + x;
-        }
-        __syncthreads();
-        if (lane == 0) warp_red[tid >> 5] = v;
-        __syncthreads();
-        v = warp_red[0];
+            for (uint32_t i = 0; i < kAhead; ++i)
+                y[i] = k + i < n ? *reinterpret_cast<const float4 *>(po + (uint64_t)(k + i) * kRows * D)
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 1; w < kJoinThreads / 32; ++w) v = take_max ? fmaxf(v, warp_red[w]) : v + warp_red[w];
-        return v;
-    };
-    const uint32_t way = tid / kLanes;
-    const uint64_t pitch = (uint64_t)pitch_rows * D;
-    // one row per CTA unless the tile has more than the launch expected
-    for (uint32_t r = r0; row0 + r < row_end; r += tile_rows) {
-        const float2 *ml = part.ml + (uint64_t)r * launched;
-        float m = -INFINITY;
-        for (uint32_t k = tid; k < n; k += kJoinThreads) m = fmaxf(m, ml[k].x);
-        m = all(m, true);
-        const uint32_t row = row0 + r, token = rq.first + row / G, qh = head * G + row % G;
-        for (uint32_t f0 = chunk * 64; f0 < D; f0 += chunks * 64) {
-            const uint32_t f = f0 + tid % kLanes * 4;
-            const float *po = part.o + (uint64_t)r * D + f;
-            float l = 0.0f;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (uint32_t k0 = 0; k0 < n; k0 += kBatch) {
-                const uint32_t count = min(n - k0, kBatch);
-                __syncthreads();
-                for (uint32_t k = tid; k < count; k += kJoinThreads) {
-                    const float2 x = ml[k0 + k];
-                    const float w = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - m);
-                    weight[k] = w;
-                    l += x.y * w;
-                }
-                __syncthreads();
-                for (uint32_t k = way; k < count; k += kWays * kAhead) {
-                    float4 y[kAhead];
-#pragma unroll
-                    for (uint32_t i = 0; i < kAhead; ++i)
-                        y[i] = k + i * kWays < count ? *reinterpret_cast<const float4 *>(po + (k0 + k + i * kWays) * pitch)
-                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                    for (uint32_t i = 0; i < kAhead; ++i) {
-                        const float w = k + i * kWays < count ? weight[k + i * kWays] : 0.0f;
-                        o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
-                    }
-                }
-            }
-            l = all(l, false);
-            way_sum[way][tid % kLanes] = o;
-            __syncthreads();
-            if (way == 0) {
-#pragma unroll
-                for (uint32_t w = 1; w < kWays; ++w) {
-                    const float4 y = way_sum[w][tid];
-                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
-                }
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-                if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY))
-                    raise(err, kErrNonFinite);
-                store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
-                if (a.lse != nullptr && f == 0)
-                    a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const float2 x = k + i < n ? ml[k + i] : make_float2(-INFINITY, 0.0f);
+                const float w = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - m);
+                l += x.y * w;
+                o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
             }
         }
+        finish4<BF16>(a, rq, G, head, row0 + r, f, D, m, l, o, err);
     }
 }
 
@@ -1036,22 +1298,32 @@ namespace {
 
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kShortRows = 64;        // requests up to this many rows go to the row kernel
-constexpr uint32_t kMaxRowGroups = 128;    // 32 groups to a warp: one batch of page ids
-constexpr uint32_t kMinRowGroups = 8;
+constexpr uint32_t kManyPartials = 8;      // a tile cut this often is joined by many CTAs
 constexpr uint32_t kMinPromptGroups = 64;
 
-template <int D, int MODE, bool E4M3>
+template <int D, int NT, bool BF16, bool E4M3>
 void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
                  cudaStream_t stream) {
+    constexpr int TERMS = BF16 ? 1 : 2;
     static DeviceOnce once;
     once.run([] {
-        cudaFuncSetAttribute(kv8_rows_kernel<D, MODE, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kRowSmem<D, terms_of(MODE)>);
+        cudaFuncSetAttribute(kv8_rows_kernel<D, NT, TERMS, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kRowSmem<D, NT, TERMS>);
     });
-    KernelTimer timer("kv8_rows", stream);
-    launch_pdl(kv8_rows_kernel<D, MODE, E4M3>, s.requests * h.row_tiles * c.heads * h.row_splits, kRowWarps * 32,
-               kRowSmem<D, terms_of(MODE)>, stream, c, s, a, h, err);
-    count_launch();
+    {
+        KernelTimer timer("kv8_rows", stream);
+        launch_pdl(kv8_rows_kernel<D, NT, TERMS, E4M3>, h.row_shares, kRowThreads, kRowSmem<D, NT, TERMS>, stream, c, s, a, h,
+                   err);
+        count_launch();
+    }
+    if (h.row_shares > 1) {
+        if (h.join_wide)
+            launch_pdl(kv8_rows_join_kernel<D, NT, BF16, true>, h.row_shares * 8 * NT * (D / 64), kShareJoinThreads, 0,
+                       stream, c, s, a, h, err);
+        else
+            launch_pdl(kv8_rows_join_kernel<D, NT, BF16, false>, h.row_shares, kShareJoinThreads, 0, stream, c, s, a, h, err);
+        count_launch();
+    }
 }
 
 template <int D, bool BF16, bool E4M3>
@@ -1071,21 +1343,13 @@ void launch_all(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const K
             count_launch();
         }
         if (h.prompt_splits > 1) {
-            launch_pdl(kv8_join_kernel<D, BF16>, h.prompt_tiles * c.heads * h.prompt_rows, kJoinThreads, 0, stream, c, s, a,
-                       h, 1u, err);
+            launch_pdl(kv8_prompt_join_kernel<D, BF16>, h.prompt_tiles * c.heads * (h.prompt_rows / 16), kJoinThreads, 0,
+                       stream, c, s, a, h, err);
             count_launch();
         }
     }
-    if constexpr (BF16)
-        launch_rows<D, kPlain, E4M3>(c, s, a, h, err, stream);
-    else
-        h.row_tile == 8 ? launch_rows<D, kStacked, E4M3>(c, s, a, h, err, stream)
-                        : launch_rows<D, kTwoTerm, E4M3>(c, s, a, h, err, stream);
-    if (h.row_splits > 1) {
-        launch_pdl(kv8_join_kernel<D, BF16>, s.requests * h.row_tiles * c.heads * h.join_rows * h.join_chunks, kJoinThreads,
-                   0, stream, c, s, a, h, 0u, err);
-        count_launch();
-    }
+    h.row_tile == 8 ? launch_rows<D, 1, BF16, E4M3>(c, s, a, h, err, stream)
+                    : launch_rows<D, 2, BF16, E4M3>(c, s, a, h, err, stream);
 }
 
 template <int D>
@@ -1101,8 +1365,7 @@ uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16,
-                          uint64_t max_kv_length) {
+Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length) {
     Kv8Shape h{};
     const uint64_t G = query_heads / c.heads;
     const uint64_t room = (uint64_t)s.columns * c.page_tokens;
@@ -1111,18 +1374,17 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
     // the longest request, if every request brings a token
     const uint64_t longest = (s.tokens > s.requests ? s.tokens - s.requests : 0) + 1, rows = longest * G;
     const bool prompts = rows > kShortRows;
-    h.row_tiles = (uint32_t)ceil_div(std::min<uint64_t>(rows, kShortRows), 16);
     h.row_limit = prompts ? kShortRows : UINT32_MAX;
-    h.row_tile = !bf16 && rows <= 8 ? 8 : 16;
-    // about two waves of two CTAs per SM if every request were the deepest
-    const uint64_t items = (uint64_t)s.requests * h.row_tiles * c.heads;
-    uint64_t each = ceil_div(items * groups, 4 * kSms);
-    each = std::min<uint64_t>(kMaxRowGroups, std::max<uint64_t>(kMinRowGroups, each));
-    h.row_groups = (uint32_t)each;
-    h.row_splits = (uint32_t)std::min<uint64_t>(ceil_div(groups, each), 4096);
-    h.join_rows = (uint32_t)std::min<uint64_t>(rows, 16);
-    h.join_chunks = items * h.join_rows < kSms ? c.dim / 64 : 1u;
-    h.row_floats = h.row_splits > 1 ? items * h.row_splits * 16 * (c.dim + 2) : 0;
+    h.row_tile = rows <= 8 ? 8 : 16;
+    // one wave of the row kernel, or shares of at least kMinShare groups
+    const uint64_t tiles = ceil_div(std::min<uint64_t>(rows, kShortRows), h.row_tile);
+    const uint64_t items = s.requests * tiles * c.heads;
+    const uint32_t wide = h.row_tile / 8 * c.dim;
+    const uint64_t wave = kSms * (wide == 512 ? 2 : c.dim == 256 || wide == 256 ? 3 : 4);
+    h.row_shares = (uint32_t)std::min<uint64_t>(wave, std::max<uint64_t>(1, items * groups / kMinShare));
+    h.join_wide = h.row_shares / items >= kManyPartials;
+    h.row_floats = h.row_shares > 1 ? 2ull * h.row_shares * h.row_tile * (c.dim + 2) + 4ull * h.row_shares : 0;
+    h.row_floats = ceil_div(h.row_floats, 4) * 4;   // what follows is read 16 bytes at a time
     h.prompt_rows = c.dim == 256 ? kPromptRows<256> : c.dim == 128 ? kPromptRows<128> : kPromptRows<64>;
     if (prompts) {
         h.prompt_tiles = (uint32_t)((uint64_t)s.tokens * G / h.prompt_rows + s.requests);
