@@ -35,6 +35,7 @@ SOURCES = [
     "kernels_layer.cu",
     "kernels_kv8.cu",
     "kernels_kv8_attend.cu",
+    "kernels_kv8_prompt.cu",
     "runtime.cpp",
     "api_basic.cpp",
     "api_provider.cpp",

@@ -143,13 +143,13 @@ kq_status row_bytes(uint32_t tokens, uint64_t stride, uint64_t width, uint32_t s
 }
 
 // Query heads against the cache, and the launch sizes; `shape` cuts the work.
-kq_status check_attend(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length,
+kq_status check_attend(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16, uint64_t max_kv_length,
                        Kv8Shape *shape, kq_diagnostic *d) {
     if (query_heads == 0 || query_heads % c.heads != 0)
         return fail(d, KQ_STATUS_DIMENSION_MISMATCH, "query heads must be a multiple of the key/value heads");
     if ((uint64_t)s.tokens * (query_heads / c.heads) > INT32_MAX)
         return fail(d, KQ_STATUS_LIMIT_EXCEEDED, "a step has at most 2^31 - 1 query rows per key/value head");
-    *shape = kv8_attend_shape(c, s, query_heads, max_kv_length);
+    *shape = kv8_attend_shape(c, s, query_heads, bf16, max_kv_length);
     const uint64_t prompt = (uint64_t)shape->prompt_tiles * c.heads *
                             std::max<uint64_t>(shape->prompt_splits, shape->prompt_rows);
     if (prompt > INT32_MAX)
@@ -271,11 +271,15 @@ kq_status kq_b200_kv8_attend_workspace_bytes(const kq_b200_kv8_cache *cache, con
     if (bytes == nullptr) return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "a result is required");
     Kv8Cache c;
     Kv8Step s;
-    Kv8Shape shape;
+    Kv8Shape shape{};
     kq_status st = check_cache(cache, false, &c, diagnostic);
     if (st == KQ_STATUS_OK) st = check_step(step, &s, diagnostic);
-    if (st == KQ_STATUS_OK) st = check_attend(c, s, query_heads, max_kv_length, &shape, diagnostic);
-    if (st == KQ_STATUS_OK) *bytes = 4 * (shape.row_floats + shape.prompt_floats);
+    uint64_t most = 0;
+    for (int bf16 = 0; bf16 < 2 && st == KQ_STATUS_OK; ++bf16) {   // enough for either type
+        st = check_attend(c, s, query_heads, bf16 != 0, max_kv_length, &shape, diagnostic);
+        most = std::max(most, 4 * (shape.row_floats + shape.prompt_floats));
+    }
+    if (st == KQ_STATUS_OK) *bytes = most;
     return st;
 }
 
@@ -289,7 +293,8 @@ kq_status kq_b200_kv8_attend(const kq_b200_kv8_cache *cache, const kq_b200_kv8_s
     Kv8Shape shape;
     kq_status st = check_cache(cache, true, &c, diagnostic);
     if (st == KQ_STATUS_OK) st = check_step(step, &s, diagnostic);
-    if (st == KQ_STATUS_OK) st = check_attend(c, s, query_heads, max_kv_length, &shape, diagnostic);
+    if (st == KQ_STATUS_OK)
+        st = check_attend(c, s, query_heads, dtype == KQ_B200_KV8_BF16, max_kv_length, &shape, diagnostic);
     if (st != KQ_STATUS_OK) return st;
     if (!known_dtype(dtype)) return fail(diagnostic, KQ_STATUS_UNSUPPORTED_TENSOR_TYPE, "queries are F32 or BF16");
     if (!std::isfinite(softmax_scale)) return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "softmax scale must be finite");

@@ -60,13 +60,17 @@ struct Kv8Shape {
     uint64_t row_floats, prompt_floats;   // workspace
 };
 
-Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length);
+Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16,
+                          uint64_t max_kv_length);
+uint32_t kv8_prompt_rows(uint32_t dim, bool bf16);
 
 void launch_kv8_plan(const Kv8Cache &c, const Kv8Step &s, const Kv8Plan &p, ErrorWord err, cudaStream_t stream);
 void launch_kv8_append(const Kv8Cache &c, const Kv8Step &s, const void *k, uint64_t k_stride, const void *v,
                        uint64_t v_stride, uint32_t bf16, ErrorWord err, cudaStream_t stream);
 void launch_kv8_read(const Kv8Cache &c, const int32_t *pages, uint32_t count, float *out, ErrorWord err,
                      cudaStream_t stream);
+void launch_kv8_prompt(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &shape, ErrorWord err,
+                       cudaStream_t stream);
 void launch_kv8_attend(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &shape, ErrorWord err,
                        cudaStream_t stream);
 

@@ -9,9 +9,8 @@
 // tiles that read the same codes.
 //
 // Products.  Codes convert to fp16 exactly (int8: |code| <= 127; e4m3: 4
-// significant bits, exponents -9..8), so the products run on
-// mma.sync.m16n8k16 with fp16 operands and F32 accumulators: S = Q K^T with
-// rows of Q as the M side, O = P V with the S accumulators as its A operand.
+// significant bits, exponents -9..8), so the products S = Q K^T and O = P V
+// run on the tensor cores with fp16 operands and F32 accumulators.
 // A row of Q is scaled by an exact power of two so that its largest element
 // lies in [2^13, 2^14): bfloat16 queries are then exact in fp16 (elements
 // 2^-27 below the row's largest lose bits, below F32's own rounding of the
@@ -44,375 +43,23 @@
 //            units, whatever the requests' lengths; a tile that spans shares
 //            leaves (m, l, O) partials which a second kernel joins in order.
 //            HBM bound: every (request, head) reads its codes once.
-//   prompt   8 warps of 16 or 32 rows each (the M side) share every group of
-//            codes; a ninth warp keeps the ring full.  Bound by the tensor
-//            pipe and the instructions that feed it.
+//   prompt   tcgen05 tiles of 128 rows (kernels_kv8_prompt.cu).
 // Partials are joined in a fixed order: results do not depend on timing.
-#include "kernels_kv8.hpp"
+#include "kernels_kv8.cuh"
 
 #include <algorithm>
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace kqb {
 
 namespace {
-
-constexpr uint32_t kG = kKv8GroupTokens;
-constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kRaise = 8.0f;        // a logit this far above m raises it
-constexpr float kWeightScale = 64.0f; // 2^6
-constexpr uint32_t kWaitPolls = 1u << 22;
-
-__device__ __forceinline__ bool err_raised(const ErrorWord &e) {
-    return *reinterpret_cast<volatile unsigned long long *>(e.word) != 0ull;
-}
-
-__device__ __forceinline__ void raise(const ErrorWord &e, uint32_t code) {
-    atomicCAS(e.word, 0ull, ((unsigned long long)code << 32) | e.call_id);
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void bulk_copy(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-
-__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// Bounded wait for the phase of `bar` with the given parity.
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
-    const uint32_t a = smem_u32(bar);
-    for (uint32_t i = 0; i < kWaitPolls; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ void mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// What fp16 rounding of (lo, hi) left behind, as fp16.
-__device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packed) {
-    const __half2 h = *reinterpret_cast<const __half2 *>(&packed);
-    return pack_half(lo - __low2float(h), hi - __high2float(h));
-}
-
-// Four stored bytes -> two fp16 pairs, exactly.  int8: each byte becomes the
-// low mantissa bits of 1024 (one PRMT per pair), and 1024 + 128 come off.
-template <bool E4M3>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t &b0, uint32_t &b1) {
-    if constexpr (E4M3) {
-        asm("{\n\t.reg .b16 x, y;\n\t"
-            "mov.b32 {x, y}, %2;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %0, x;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
-            : "=r"(b0), "=r"(b1)
-            : "r"(w));
-    } else {
-        const uint32_t c = 0x64646464u;
-        const uint32_t x = __byte_perm(w, c, 0x4140), y = __byte_perm(w, c, 0x4342);
-        const __half2 bias = __half2(__ushort_as_half(0xE480), __ushort_as_half(0xE480));   // -1152
-        const __half2 u = __hadd2(*reinterpret_cast<const __half2 *>(&x), bias);
-        const __half2 v = __hadd2(*reinterpret_cast<const __half2 *>(&y), bias);
-        b0 = *reinterpret_cast<const uint32_t *>(&u);
-        b1 = *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
-
-// The key/value groups that the rows of one tile can see, and where its
-// request stands.
-struct Request {
-    uint32_t first, n, length;   // first query token, query tokens, cached tokens (new ones included)
-};
-
-// Reads and checks request b of the step; false (and an error) if its entries
-// are out of range.
-__device__ __forceinline__ bool load_request(const Kv8Cache &c, const Kv8Step &s, uint32_t b, Request &r,
-                                             const ErrorWord &err) {
-    const int32_t o0 = s.query_offsets[b], o1 = s.query_offsets[b + 1], len = s.kv_lengths[b];
-    const bool ok = o0 >= 0 && o1 >= o0 && (uint32_t)o1 <= s.tokens && len >= 0 &&
-                    (uint64_t)len <= (uint64_t)s.columns * c.page_tokens;
-    r.first = (uint32_t)o0;
-    r.n = (uint32_t)(o1 - o0);
-    r.length = (uint32_t)len;
-    if (!ok) raise(err, kErrStep);
-    return ok;
-}
-
-// One tile per warp and MT: softmax state and accumulators.  Thread (g, t) =
-// (lane / 4, lane % 4) holds rows g and g + 8.
-template <int D, int MT>
-struct Rows {
-    float o[MT][D / 8][4];
-    float m[MT][2], l[MT][2], ref;
-
-    __device__ __forceinline__ void clear() {
-        ref = 0.0f;
-#pragma unroll
-        for (int a = 0; a < MT; ++a) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) m[a][h] = -INFINITY, l[a][h] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[a][n][k] = 0.0f;
-        }
-    }
-};
-
-// One step over NG groups of 16 consecutive tokens each (`kv`: their codes in
-// shared memory, 32 * D bytes a group).  q: the rows' fragments
-// [MT][TERMS][D / 16][32 lanes].  factor: per row, softmax scale * log2 e /
-// the row's power of two.  limit: last visible token per row (-1: none);
-// compared only when MASK.
-// The first product's sums run in CH chains where a warp has few tiles: a
-// chain of dependent MMAs waits for each one.
-template <int D, int MT, int NG, int TERMS, bool E4M3, bool MASK>
-__device__ __forceinline__ void group_step(Rows<D, MT> &st, const uint4 *q, const uint8_t *kv, const float (&ks)[NG],
-                                           const float (&vs)[NG], const float (&factor)[MT][2],
-                                           const int32_t (&limit)[MT][2], int32_t token, uint32_t lane) {
-    constexpr int CH = MT * NG >= 4 ? 1 : 4 / (MT * NG);
-    float s[MT][NG][2][4];
-    {
-        float c[CH][MT][NG][2][4];
-#pragma unroll
-        for (int x = 0; x < CH; ++x)
-#pragma unroll
-            for (int a = 0; a < MT; ++a)
-#pragma unroll
-                for (int n = 0; n < NG; ++n)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) c[x][a][n][h][k] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-            uint4 w[NG][2];
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w[n][h] = *reinterpret_cast<const uint4 *>(kv + n * 32 * D + j * 1024 + h * 512 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t b[NG][2][2];
-#pragma unroll
-                for (int n = 0; n < NG; ++n)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint4 &x = w[n][h];
-                        widen<E4M3>(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, b[n][h][0], b[n][h][1]);
-                    }
-#pragma unroll
-                for (int a = 0; a < MT; ++a)
-#pragma unroll
-                    for (int term = TERMS - 1; term >= 0; --term) {
-                        const uint4 f = q[((a * TERMS + term) * (D / 16) + j * 4 + i) * 32 + lane];
-#pragma unroll
-                        for (int n = 0; n < NG; ++n)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                mma(c[(i * TERMS + term) % CH][a][n][h], f, b[n][h][0], b[n][h][1]);
-                    }
-            }
-        }
-#pragma unroll
-        for (int a = 0; a < MT; ++a)
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float v = c[0][a][n][h][k];
-#pragma unroll
-                        for (int x = 1; x < CH; ++x) v += c[x][a][n][h][k];
-                        s[a][n][h][k] = v;
-                    }
-    }
-
-    // logits, the rows' maxima
-    float top[MT][2];
-    bool lift = false;
-#pragma unroll
-    for (int a = 0; a < MT; ++a) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float x = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                const float f = factor[a][r] * ks[n];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        float v = s[a][n][h][2 * r + k] * f;
-                        if (MASK && token + n * 16 + h * 8 + (int32_t)(lane & 3) * 2 + k > limit[a][r]) v = -INFINITY;
-                        s[a][n][h][2 * r + k] = v;
-                        x = fmaxf(x, v);
-                    }
-            }
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
-            x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
-            top[a][r] = x;
-            lift |= x > st.m[a][r] + kRaise;
-        }
-    }
-    if (__any_sync(~0u, lift)) {   // -inf + 8 is -inf: the first finite logit of a row lifts it
-#pragma unroll
-        for (int a = 0; a < MT; ++a) {
-            float by[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float m = fmaxf(st.m[a][r], top[a][r]);
-                by[r] = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
-                st.m[a][r] = m;
-                st.l[a][r] *= by[r];
-            }
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by[k >> 1];
-        }
-    }
-    float most = vs[0];
-#pragma unroll
-    for (int n = 1; n < NG; ++n) most = fmaxf(most, vs[n]);
-    if (most > st.ref) {
-        // the next power of two, within the normal range
-        const uint32_t e = min((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
-        const float ref = __uint_as_float(max(e, 0x00800000u));
-        const float by = st.ref / ref;
-        st.ref = ref;
-#pragma unroll
-        for (int a = 0; a < MT; ++a)
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by;
-    }
-    const float inv = st.ref > 0.0f ? kWeightScale / st.ref : 0.0f;
-
-    // weights, as the second product's A operand
-    uint4 p[MT][NG][TERMS];
-#pragma unroll
-    for (int a = 0; a < MT; ++a) {
-        float m[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) m[r] = st.m[a][r] == -INFINITY ? 0.0f : st.m[a][r];
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            const float w = vs[n] * inv;
-            float e[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    e[h][k] = exp2_approx(s[a][n][h][k] - m[k >> 1]);
-                    st.l[a][k >> 1] += e[h][k];
-                    e[h][k] *= w;
-                }
-            }
-            p[a][n][0] = make_uint4(pack_half(e[0][0], e[0][1]), pack_half(e[0][2], e[0][3]), pack_half(e[1][0], e[1][1]),
-                                    pack_half(e[1][2], e[1][3]));
-            if constexpr (TERMS == 2)
-                p[a][n][1] = make_uint4(pack_rest(e[0][0], e[0][1], p[a][n][0].x), pack_rest(e[0][2], e[0][3], p[a][n][0].y),
-                                        pack_rest(e[1][0], e[1][1], p[a][n][0].z), pack_rest(e[1][2], e[1][3], p[a][n][0].w));
-        }
-    }
-
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-        uint4 w[NG];
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-            w[n] = *reinterpret_cast<const uint4 *>(kv + n * 32 * D + 16 * D + j * 512 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t b[NG][2];
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-                widen<E4M3>(i == 0 ? w[n].x : i == 1 ? w[n].y : i == 2 ? w[n].z : w[n].w, b[n][0], b[n][1]);
-#pragma unroll
-            for (int a = 0; a < MT; ++a) {
-                if constexpr (TERMS == 2) {
-                    // a fresh accumulator per step, added in F32: the tensor
-                    // core's own addition truncates, and over thousands of
-                    // groups that bias would exceed F32's rounding
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        mma(d, p[a][n][1], b[n][0], b[n][1]);
-                        mma(d, p[a][n][0], b[n][0], b[n][1]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) st.o[a][j * 4 + i][k] += d[k];
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) mma(st.o[a][j * 4 + i], p[a][n][0], b[n][0], b[n][1]);
-                }
-            }
-        }
-    }
-}
-
-// Four query elements from element `at` on.
-template <bool BF16>
-__device__ __forceinline__ float4 load4(const void *base, uint64_t at) {
-    if constexpr (BF16) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(base) + at);
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                           __uint_as_float(w.y & 0xffff0000u));
-    } else {
-        return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-    }
-}
 
 // Writes ROWS rows from row0 of request `rq` as fragments into q and, per row,
 // 1 / its power of two (times the softmax scale in base 2) into factor and its
 // last visible token into limit.  Eight threads per row, every thread of the
 // CTA takes part; rows behind the request's last are zero with limit -1.
 // Returns whether a query value was not finite.
-// COLUMNS: the rows are the products' N side, fragments
-// [8-row tile][TERMS][D / 16][32 lanes][2]; else their M side,
-// [16-row tile][TERMS][D / 16][32 lanes][4].
-template <int D, int TERMS, bool COLUMNS, int THREADS, int ROWS>
+// The rows are the products' N side: [8-row tile][TERMS][D / 16][32 lanes][2].
+template <int D, int TERMS, int THREADS, int ROWS>
 __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &rq, uint32_t G, uint32_t head,
                                              uint32_t row0, void *q, float *factor, int32_t *limit, uint32_t tid) {
     bool bad = false;
@@ -447,20 +94,12 @@ __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &
             const uint32_t f = (part + 8 * k) * 4, step = f / 64 * 4 + f % 16 / 4, lane = (r & 7) * 4 + f % 64 / 16;
             const float a0 = x[k].x * up, a1 = x[k].y * up, a2 = x[k].z * up, a3 = x[k].w * up;
             const uint32_t h0 = pack_half(a0, a1), h1 = pack_half(a2, a3);
-            // places of the pair (features f, f + 1), of the next pair and of the low terms
-            uint32_t at, next, low;
-            if constexpr (COLUMNS) {
-                at = (((r >> 3) * TERMS * (D / 16) + step) * 32 + lane) * 2;
-                next = 1, low = D / 16 * 64;
-            } else {
-                at = (((r >> 4) * TERMS * (D / 16) + step) * 32 + lane) * 4 + (r >> 3 & 1);
-                next = 2, low = D / 16 * 128;
-            }
+            const uint32_t at = (((r >> 3) * TERMS * (D / 16) + step) * 32 + lane) * 2;
             q32[at] = h0;
-            q32[at + next] = h1;
+            q32[at + 1] = h1;
             if constexpr (TERMS == 2) {
-                q32[at + low] = pack_rest(a0, a1, h0);
-                q32[at + low + next] = pack_rest(a2, a3, h1);
+                q32[at + D / 16 * 64] = pack_rest(a0, a1, h0);
+                q32[at + D / 16 * 64 + 1] = pack_rest(a2, a3, h1);
             }
         }
         if (part == 0) {
@@ -469,57 +108,6 @@ __device__ __forceinline__ bool load_queries(const Kv8Attend &a, const Request &
         }
     }
     return bad;
-}
-
-// A finished row's value and its log-sum, or a split's partial.
-template <bool BF16>
-__device__ __forceinline__ void store4(void *out, uint64_t at, float4 v) {
-    if constexpr (BF16) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(out) + at) =
-            make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
-    } else {
-        *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = v;
-    }
-}
-
-// Four features of a row from its sums: the output and, with the first four,
-// the log-sum.
-template <bool BF16>
-__device__ __forceinline__ void finish4(const Kv8Attend &a, const Request &rq, uint32_t G, uint32_t head, uint32_t row,
-                                        uint32_t f, uint32_t dim, float m, float l, float4 o, const ErrorWord &err) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-    if (!(l < INFINITY) || !(fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY)) raise(err, kErrNonFinite);
-    const uint64_t token = rq.first + row / G;
-    const uint32_t qh = head * G + row % G;
-    store4<BF16>(a.out, token * a.out_stride + (uint64_t)qh * dim + f, o);
-    if (a.lse != nullptr && f == 0) a.lse[token * a.query_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
-}
-
-// Where the partials of a (tile, head) lie: O [split][row][D], and behind the
-// O of all `tiles`, (m, l) [row][split].
-struct Partials {
-    float *o;
-    float2 *ml;
-    __device__ __forceinline__ Partials(float *base, uint64_t tile, uint32_t splits, uint32_t rows, uint32_t dim,
-                                        uint64_t tiles) {
-        o = base + tile * splits * rows * dim;
-        ml = reinterpret_cast<float2 *>(base + tiles * splits * rows * dim) + tile * rows * splits;
-    }
-};
-
-// Groups of 16 tokens that the rows up to `last_row` of a request see.
-__device__ __forceinline__ uint32_t visible_groups(const Request &rq, uint32_t G, uint32_t rows_end) {
-    const uint32_t token = (rows_end - 1) / G;   // the tile's last token
-    const int64_t last = (int64_t)rq.length - rq.n + min(token, rq.n - 1);
-    return last < 0 ? 0u : (uint32_t)(last / kG) + 1u;
-}
-
-// A split's groups: at least `each`, never more splits than the launch has,
-// and whole stages (`unit` groups, which `each` is a multiple of).
-__device__ __forceinline__ uint32_t split_groups(uint32_t groups, uint32_t each, uint32_t splits, uint32_t unit) {
-    return max(each, ((groups + splits - 1) / splits + unit - 1) / unit * unit);
 }
 
 // ------------------------------------------------------------------- rows
@@ -832,7 +420,7 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
         for (; issued < min(mine, (uint32_t)ST); ++issued) issue(issued, 0);
         fetch(32, 1);
 
-        if (load_queries<D, TERMS, true, kRowThreads, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
+        if (load_queries<D, TERMS, kRowThreads, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
             raise(err, kErrNonFinite);
         __syncthreads();
         Columns<D, NT> st;
@@ -1029,227 +617,21 @@ kv8_rows_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWo
     }
 }
 
+// ------------------------------------------------------------ prompt join
+
 namespace {
 
-// ----------------------------------------------------------------- prompt
-
-constexpr int kPromptWarps = 8;
-constexpr int kPromptThreads = (kPromptWarps + 4) * 32;
-constexpr int kPromptGroups = 2;   // groups per ring stage
-template <int D> constexpr int kPromptMt = D == 256 ? 1 : 2;
-template <int D> constexpr uint32_t kPromptRows = kPromptWarps * 16 * kPromptMt<D>;
-template <int D> constexpr int kPromptStages = D == 256 ? 4 : 8;
-template <int D, int TERMS>
-constexpr uint32_t kPromptSmem = kPromptStages<D> * kPromptGroups * 32 * D + kPromptRows<D> * D * 2 * TERMS;
-
-// The request and tile of compact tile index t: request b's tiles begin at
-// floor(offset_b * G / rows) + b, which leaves room for its partial tile.
-// The warp searches 32 ways at a time.
-__device__ __forceinline__ uint32_t find_request(const Kv8Step &s, uint32_t G, uint32_t tile_rows, uint32_t t,
-                                                 uint32_t lane, uint32_t &start) {
-    uint32_t lo = 0, n = s.requests;   // the answer lies in [lo, lo + n)
-    auto begin = [&](uint32_t b) {
-        return (uint32_t)((uint64_t)(uint32_t)max(s.query_offsets[b], 0) * G / tile_rows) + b;
-    };
-    while (n > 1) {
-        const uint32_t step = (n + 31) / 32, at = lo + lane * step;
-        const bool in = lane * step < n && begin(at) <= t;
-        const uint32_t hits = __ballot_sync(~0u, in);
-        const uint32_t k = hits ? 31 - __clz(hits) : 0u;
-        const uint32_t end = lo + n;
-        lo += k * step;
-        n = min(step, end - lo);
-    }
-    start = begin(lo);
-    return lo;
-}
+constexpr int kJoinThreads = 256;
 
 }  // namespace
-
-// grid (tile, head, split), the last tiles first (they see the most tokens).
-// Warp w < 8 holds rows [16 MT w, 16 MT (w + 1)) of the tile; warp 8 streams
-// the split's groups, two to a stage, and leaves their scales beside them.
-// Registers: 384 threads of 168 at launch (64,512); the consumers' two
-// warpgroups take 232 each thread, the producer's keeps 40 (the same sum).
-template <int D, bool BF16, bool E4M3>
-__global__ void __launch_bounds__(kPromptThreads, 1)
-kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr int TERMS = BF16 ? 1 : 2, MT = kPromptMt<D>, ST = kPromptStages<D>, NG = kPromptGroups;
-    constexpr uint32_t kGroup = 32 * D, kStage = NG * kGroup, kRows = kPromptRows<D>;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t full[ST], empty[ST];
-    __shared__ float2 stage_scales[ST][NG];
-    __shared__ float factor_s[kRows];
-    __shared__ int32_t limit_s[kRows];
-    __shared__ int gave_up;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint4 *q = reinterpret_cast<uint4 *>(smem + ST * kStage);
-    const uint32_t G = a.query_heads / c.heads;
-    const uint32_t split = blockIdx.x % shape.prompt_splits, u = blockIdx.x / shape.prompt_splits;
-    const uint32_t head = u % c.heads, t = shape.prompt_tiles - 1 - u / c.heads;
-
-    if (tid == 0) {
-        gave_up = 0;
-        for (int k = 0; k < ST; ++k) {
-            bar_init(&full[k], NG);
-            bar_init(&empty[k], kPromptWarps);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    pdl_wait();
-    if (__syncthreads_or(tid == 0 && err_raised(err))) return;
-    uint32_t start;
-    const uint32_t b = find_request(s, G, kRows, t, lane, start);
-    Request rq;
-    if (!load_request(c, s, b, rq, err)) return;
-    const uint64_t rows64 = (uint64_t)rq.n * G;
-    if (t < start || rows64 <= shape.row_limit || (uint64_t)(t - start) * kRows >= rows64) return;
-    const uint32_t rows = (uint32_t)rows64, row0 = (t - start) * kRows, row_end = min(row0 + kRows, rows);
-    const uint32_t groups = visible_groups(rq, G, row_end), each = split_groups(groups, shape.prompt_groups, shape.prompt_splits, NG);
-    const uint32_t g0 = split * each, g1 = min(g0 + each, groups);
-    if (split > 0 && g0 >= groups) return;
-    const uint32_t stages = g1 > g0 ? (g1 - g0 + NG - 1) / NG : 0u;
-    volatile int *quit = &gave_up;
-
-    if (warp >= kPromptWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        // producer: lane k < NG of warp 8 brings group k of every stage (behind
-        // an odd last group that group again: its tokens are behind every
-        // row's limit then)
-        bool ok = true;
-        uint32_t done = 0;
-        if (warp == kPromptWarps && lane < NG) {
-            const int32_t *table = s.table + (uint64_t)b * s.table_stride;
-            const uint32_t per_page = c.page_tokens / kG;
-            const uint64_t page_bytes = 2ull * c.page_tokens * D;
-            int32_t next = stages > 0 ? table[min(g0 + lane, g1 - 1) / per_page] : 0;
-            for (uint32_t k = 0; k < stages && !*quit; ++k) {
-                const uint32_t slot = k % ST, g = min(g0 + k * NG + lane, g1 - 1);
-                const bool in = next >= 0 && (uint32_t)next < c.pages;
-                if (!in) raise(err, kErrStep);
-                const uint32_t page = in ? (uint32_t)next : 0u;   // any page: the call fails
-                if (k + 1 < stages) next = table[min(g + NG, g1 - 1) / per_page];
-                const float2 sc = *reinterpret_cast<const float2 *>(c.scales + ((uint64_t)page * c.heads + head) * 2);
-                if (k >= ST) ok = bar_wait(&empty[slot], (k / ST - 1) & 1u);
-                if (!ok) break;
-                stage_scales[slot][lane] = sc;
-                bar_expect(&full[slot], kGroup);
-                bulk_copy(smem + slot * kStage + lane * kGroup,
-                          c.codes + ((uint64_t)page * c.heads + head) * page_bytes + (uint64_t)(g % per_page) * kGroup,
-                          kGroup, &full[slot]);
-                done = k + 1;
-            }
-            if (!ok) {
-                raise(err, kErrTimeout);
-                *quit = 1;
-            }
-        }
-        __syncwarp();
-        asm volatile("bar.sync 0;" ::: "memory");
-        if (warp == kPromptWarps && lane < NG && *quit)   // copies in flight land before the CTA exits
-            for (uint32_t k = done > ST ? done - ST : 0u; k < done; ++k) bar_wait(&full[k % ST], k / ST & 1u);
-        return;
-    }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-
-    if (load_queries<D, TERMS, false, kPromptWarps * 32, kRows>(a, rq, G, head, row0, q, factor_s, limit_s, tid))
-        raise(err, kErrNonFinite);
-    asm volatile("bar.sync 1, %0;" ::"n"(kPromptWarps * 32) : "memory");
-    Rows<D, MT> st;
-    st.clear();
-    float factor[MT][2];
-    int32_t limit[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint32_t row = (warp * MT + m) * 16 + (lane >> 2) + 8 * r;
-            factor[m][r] = factor_s[row];
-            limit[m][r] = limit_s[row];
-        }
-    // tokens that every row of the warp sees, and that any does
-    const uint32_t first_row = row0 + warp * MT * 16;
-    const int64_t before = (int64_t)rq.length - rq.n;
-    const bool warp_live = first_row < row_end;
-    const int64_t all_see = warp_live && first_row + MT * 16 <= row_end ? before + first_row / G + 1 : 0;
-    const int64_t any_sees = warp_live ? before + (min(first_row + MT * 16, row_end) - 1) / G + 1 : 0;
-    const uint4 *wq = q + warp * MT * TERMS * (D / 16) * 32;
-    bool ok = true;
-    for (uint32_t k = 0; k < stages; ++k) {
-        const uint32_t slot = k % ST;
-        ok = !*quit && bar_wait(&full[slot], k / ST & 1u);
-        if (!ok) break;
-        const int64_t token = (int64_t)(g0 + k * NG) * kG;
-        if (token < any_sees) {
-            const float2 s0 = stage_scales[slot][0], s1 = stage_scales[slot][1];
-            const float ks[NG] = {s0.x, s1.x}, vs[NG] = {s0.y, s1.y};
-            const uint8_t *kv = smem + slot * kStage;
-            if (token + NG * kG > all_see || g0 + (k + 1) * NG > g1)
-                group_step<D, MT, NG, TERMS, E4M3, true>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
-            else
-                group_step<D, MT, NG, TERMS, E4M3, false>(st, wq, kv, ks, vs, factor, limit, (int32_t)token, lane);
-        }
-        __syncwarp();
-        if (lane == 0) bar_arrive(&empty[slot]);
-    }
-    if (!ok) {
-        if (lane == 0) {
-            *quit = 1;
-            raise(err, kErrTimeout);
-        }
-    }
-    asm volatile("bar.sync 0;" ::: "memory");
-    if (!ok) return;
-
-    const bool whole = groups <= each;
-    const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, kRows, D,
-                        (uint64_t)shape.prompt_tiles * c.heads);
-    const float back = st.ref * (1.0f / kWeightScale);
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float l = st.l[m][r];
-            l += __shfl_xor_sync(~0u, l, 1);
-            l += __shfl_xor_sync(~0u, l, 2);
-            const uint32_t in_tile = (warp * MT + m) * 16 + (lane >> 2) + 8 * r, row = row0 + in_tile;
-            if (row >= row_end) continue;
-            const uint32_t token = rq.first + row / G, qh = head * G + row % G;
-            const float by = whole ? (l > 0.0f ? back / l : 0.0f) : back;
-            bool fine = l < INFINITY;
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float4 o = make_float4(st.o[m][4 * j][2 * r + k] * by, st.o[m][4 * j + 1][2 * r + k] * by,
-                                                 st.o[m][4 * j + 2][2 * r + k] * by, st.o[m][4 * j + 3][2 * r + k] * by);
-                    const uint32_t f = j * 32 + (lane & 3) * 8 + 4 * k;
-                    if (whole) {
-                        fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
-                        store4<BF16>(a.out, (uint64_t)token * a.out_stride + (uint64_t)qh * D + f, o);
-                    } else {
-                        *reinterpret_cast<float4 *>(part.o + ((uint64_t)split * kRows + in_tile) * D + f) = o;
-                    }
-                }
-            if ((lane & 3) == 0) {
-                if (!whole)
-                    part.ml[in_tile * shape.prompt_splits + split] = make_float2(st.m[m][r], l);
-                else if (a.lse != nullptr)
-                    a.lse[(uint64_t)token * a.query_heads + qh] = l > 0.0f ? (st.m[m][r] + log2f(l)) * kLn2 : -INFINITY;
-            }
-            if (whole && !fine) raise(err, kErrNonFinite);
-        }
-}
-
-constexpr int kJoinThreads = 256;
 
 // Joins the splits of a prompt tile: one CTA per (tile, head, 16 rows), a
 // thread per 4 features of a row, in split order.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads)
 kv8_prompt_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
-    constexpr uint32_t kRows = kPromptRows<D>, kAhead = 8;
-    const uint32_t tid = threadIdx.x, G = a.query_heads / c.heads;
+    constexpr uint32_t kAhead = 8;
+    const uint32_t tid = threadIdx.x, G = a.query_heads / c.heads, kRows = shape.prompt_rows;
     const uint32_t block = blockIdx.x % (kRows / 16), u = blockIdx.x / (kRows / 16), head = u % c.heads, t = u / c.heads;
     pdl_wait();
     if (__syncthreads_or(tid == 0 && err_raised(err))) return;
@@ -1261,7 +643,7 @@ kv8_prompt_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, Error
     if (rows64 <= shape.row_limit || (uint64_t)(t - start) * kRows >= rows64) return;
     const uint32_t rows = (uint32_t)rows64, row0 = (t - start) * kRows, row_end = min(row0 + kRows, rows);
     const uint32_t groups = visible_groups(rq, G, row_end);
-    const uint32_t each = split_groups(groups, shape.prompt_groups, shape.prompt_splits, kPromptGroups);
+    const uint32_t each = split_groups(groups, shape.prompt_groups, shape.prompt_splits, kPromptUnit);
     if (groups <= each) return;
     const uint32_t n = (groups + each - 1) / each;
     const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, kRows, D,
@@ -1299,7 +681,7 @@ namespace {
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kShortRows = 64;        // requests up to this many rows go to the row kernel
 constexpr uint32_t kManyPartials = 8;      // a tile cut this often is joined by many CTAs
-constexpr uint32_t kMinPromptGroups = 64;
+constexpr uint32_t kMinPromptGroups = 64;  // a split of a prompt: 1024 tokens or more
 
 template <int D, int NT, bool BF16, bool E4M3>
 void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
@@ -1329,19 +711,8 @@ void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const 
 template <int D, bool BF16, bool E4M3>
 void launch_all(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
                 cudaStream_t stream) {
-    constexpr int TERMS = BF16 ? 1 : 2;
-    static DeviceOnce once;
-    once.run([] {
-        cudaFuncSetAttribute(kv8_prompt_kernel<D, BF16, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kPromptSmem<D, TERMS>);
-    });
     if (h.prompt_tiles > 0) {
-        {
-            KernelTimer timer("kv8_prompt", stream);
-            launch_pdl(kv8_prompt_kernel<D, BF16, E4M3>, h.prompt_tiles * c.heads * h.prompt_splits, kPromptThreads,
-                       kPromptSmem<D, TERMS>, stream, c, s, a, h, err);
-            count_launch();
-        }
+        launch_kv8_prompt(c, s, a, h, err, stream);
         if (h.prompt_splits > 1) {
             launch_pdl(kv8_prompt_join_kernel<D, BF16>, h.prompt_tiles * c.heads * (h.prompt_rows / 16), kJoinThreads, 0,
                        stream, c, s, a, h, err);
@@ -1365,7 +736,8 @@ uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, uint64_t max_kv_length) {
+Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_heads, bool bf16,
+                          uint64_t max_kv_length) {
     Kv8Shape h{};
     const uint64_t G = query_heads / c.heads;
     const uint64_t room = (uint64_t)s.columns * c.page_tokens;
@@ -1385,12 +757,12 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
     h.join_wide = h.row_shares / items >= kManyPartials;
     h.row_floats = h.row_shares > 1 ? 2ull * h.row_shares * h.row_tile * (c.dim + 2) + 4ull * h.row_shares : 0;
     h.row_floats = ceil_div(h.row_floats, 4) * 4;   // what follows is read 16 bytes at a time
-    h.prompt_rows = c.dim == 256 ? kPromptRows<256> : c.dim == 128 ? kPromptRows<128> : kPromptRows<64>;
+    h.prompt_rows = kv8_prompt_rows(c.dim, bf16);
     if (prompts) {
         h.prompt_tiles = (uint32_t)((uint64_t)s.tokens * G / h.prompt_rows + s.requests);
         const uint64_t work = ceil_div((uint64_t)s.tokens * G, h.prompt_rows) * c.heads;
         const uint64_t cut = std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(2 * kSms, work), 32));
-        h.prompt_groups = (uint32_t)(ceil_div(std::max<uint64_t>(kMinPromptGroups, ceil_div(groups, cut)), kPromptGroups) * kPromptGroups);
+        h.prompt_groups = (uint32_t)(ceil_div(std::max<uint64_t>(kMinPromptGroups, ceil_div(groups, cut)), kPromptUnit) * kPromptUnit);
         h.prompt_splits = work >= kSms ? 1u : (uint32_t)ceil_div(groups, h.prompt_groups);
         h.prompt_floats = h.prompt_splits > 1
                               ? (uint64_t)h.prompt_tiles * c.heads * h.prompt_splits * h.prompt_rows * (c.dim + 2) : 0;
