@@ -53,7 +53,7 @@ struct Kv8Shape {
     uint32_t row_tile;      // rows per tile of the row kernel: 8 or 16
     uint32_t row_limit;     // requests of more rows go to the prompt kernel (UINT32_MAX: none do)
     uint32_t row_shares;    // CTAs of the row kernel
-    uint32_t join_wide;     // its cut tiles are joined by a CTA per 64 features of a row
+    uint32_t join_tiles;    // cut tiles at most, joined by a CTA per 64 features of a row (0: by a CTA per share)
     uint32_t prompt_rows;   // rows per tile of the prompt kernel
     uint32_t prompt_tiles;  // 0: the prompt kernel does not run
     uint32_t prompt_groups, prompt_splits;

@@ -539,81 +539,115 @@ constexpr int kShareJoinThreads = 256;
 
 }  // namespace
 
-// Joins the tiles that shares cut: CTA (share k, chunk) takes the tile that
-// share k began, from shares k .. last in this order.  A chunk is 64 features
-// of one row, its partials dealt to 16 groups of 16 threads (WIDE, for a few
-// tiles of many partials), or all of the tile with a thread per 4 features.
+// Joins the tiles that shares cut, from shares k (which began it) .. last in
+// this order.  Narrow: CTA k takes the tile that share k began, a thread per 4
+// features.  WIDE, for few tiles of many partials: CTA (i, chunk) takes the
+// i-th such tile, of it 64 features of one row, the partials dealt to 16
+// groups of 16 threads.
 // Bound: latency, the partials come from L2.
 template <int D, int NT, bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kShareJoinThreads)
 kv8_rows_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
     constexpr uint32_t kRows = 8 * NT, kCells = kRows * (D / 4);
     constexpr uint32_t kChunks = WIDE ? kRows * (D / 64) : 1, kWays = WIDE ? 16 : 1, kAhead = 8;
+    constexpr uint32_t kPer = 3;   // shares per thread of the search (at most 592 shares)
     __shared__ float4 way_o[kWays][WIDE ? 16 : 1];
     __shared__ float way_m[kWays], way_l[kWays];
-    const uint32_t tid = threadIdx.x, share = blockIdx.x / kChunks, chunk = blockIdx.x % kChunks;
+    __shared__ uint32_t warp_cuts[kShareJoinThreads / 32], found;
+    const uint32_t tid = threadIdx.x, chunk = blockIdx.x % kChunks;
     const uint32_t G = a.query_heads / c.heads;
     pdl_wait();
     if (__syncthreads_or(tid == 0 && err_raised(err))) return;
     const ShareSpace space(a.workspace, shape.row_shares, kRows, D);
-    const Cut cut = space.cuts[share];
-    if (cut.last <= share) return;
-    Request rq;
-    if (!load_request(c, s, cut.request, rq, err)) return;
-    const uint32_t row0 = cut.tile * kRows, row_end = min(row0 + kRows, rq.n * G), n = cut.last - share + 1;
     const uint32_t way = WIDE ? tid / 16 : 0u;
-    for (uint32_t v = WIDE ? chunk * 16 + tid % 16 : tid; v < kCells; v += WIDE ? kCells : kShareJoinThreads) {
-        const uint32_t r = v / (D / 4), f = v % (D / 4) * 4;
-        if (row0 + r >= row_end) break;
-        float m = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t k = way; k < n; k += kWays * kAhead) {
-            float4 y[kAhead];
-            float2 x[kAhead];
+    auto join = [&](uint32_t share) {   // every thread of the CTA
+        const Cut cut = space.cuts[share];
+        Request rq;
+        if (cut.last <= share || !load_request(c, s, cut.request, rq, err)) return;
+        const uint32_t row0 = cut.tile * kRows, row_end = min(row0 + kRows, rq.n * G), n = cut.last - share + 1;
+        for (uint32_t v = WIDE ? chunk * 16 + tid % 16 : tid; v < kCells; v += WIDE ? kCells : kShareJoinThreads) {
+            const uint32_t r = v / (D / 4), f = v % (D / 4) * 4;
+            if (row0 + r >= row_end) break;
+            float m = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t k = way; k < n; k += kWays * kAhead) {
+                float4 y[kAhead];
+                float2 x[kAhead];
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; ++i) {
-                const uint32_t at = k + i * kWays;
-                // the first share's partial is the one it began, the others' the one they ended or passed through
-                const uint64_t place = 2ull * (share + at) + (at == 0 ? 1 : 0);
-                const bool in = at < n;
-                y[i] = in ? *reinterpret_cast<const float4 *>(space.o + (place * kRows + r) * D + f)
-                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                x[i] = in ? space.ml[place * kRows + r] : make_float2(-INFINITY, 0.0f);
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const uint32_t at = k + i * kWays;
+                    // the first share's partial is the one it began, the others' the one they ended or passed through
+                    const uint64_t place = 2ull * (share + at) + (at == 0 ? 1 : 0);
+                    const bool in = at < n;
+                    y[i] = in ? *reinterpret_cast<const float4 *>(space.o + (place * kRows + r) * D + f)
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[i] = in ? space.ml[place * kRows + r] : make_float2(-INFINITY, 0.0f);
+                }
+                float top = m;
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].x);
+                if (top == -INFINITY) continue;
+                const float by = exp2_approx(m - top);
+                m = top;
+                l *= by, o.x *= by, o.y *= by, o.z *= by, o.w *= by;
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i) {
+                    const float w = exp2_approx(x[i].x - m);
+                    l += x[i].y * w;
+                    o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
+                }
             }
-            float top = m;
+            if constexpr (WIDE) {   // all threads are on the same row
+                way_o[way][tid % 16] = o;
+                if (tid % 16 == 0) way_m[way] = m, way_l[way] = l;
+                __syncthreads();
+                m = way_m[0];
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; ++i) top = fmaxf(top, x[i].x);
-            if (top == -INFINITY) continue;
-            const float by = exp2_approx(m - top);
-            m = top;
-            l *= by, o.x *= by, o.y *= by, o.z *= by, o.w *= by;
+                for (uint32_t w = 1; w < kWays; ++w) m = fmaxf(m, way_m[w]);
+                l = 0.0f;
+                o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; ++i) {
-                const float w = exp2_approx(x[i].x - m);
-                l += x[i].y * w;
-                o.x += y[i].x * w, o.y += y[i].y * w, o.z += y[i].z * w, o.w += y[i].w * w;
+                for (uint32_t w = 0; w < kWays; ++w) {
+                    const float by = way_m[w] == -INFINITY ? 0.0f : exp2_approx(way_m[w] - m);
+                    const float4 y = way_o[w][tid % 16];
+                    l += way_l[w] * by;
+                    o.x += y.x * by, o.y += y.y * by, o.z += y.z * by, o.w += y.w * by;
+                }
             }
+            if (way == 0) finish4<BF16>(a, rq, G, cut.head, row0 + r, f, D, m, l, o, err);
         }
-        if constexpr (WIDE) {
-            way_o[way][tid % 16] = o;
-            if (tid % 16 == 0) way_m[way] = m, way_l[way] = l;
-            __syncthreads();   // all threads of the CTA are on the same row
-            if (way > 0) return;
-            float top = way_m[0];
+    };
+    if constexpr (!WIDE) {
+        join(blockIdx.x);
+    } else {
+        uint32_t cuts = 0;
 #pragma unroll
-            for (uint32_t w = 1; w < kWays; ++w) top = fmaxf(top, way_m[w]);
-            l = 0.0f;
-            o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t k = tid * kPer; k < tid * kPer + kPer; ++k) cuts += k < shape.row_shares && space.cuts[k].last > k;
+        uint32_t before = cuts, total = 0;
 #pragma unroll
-            for (uint32_t w = 0; w < kWays; ++w) {
-                const float by = way_m[w] == -INFINITY ? 0.0f : exp2_approx(way_m[w] - top);
-                const float4 y = way_o[w][tid % 16];
-                l += way_l[w] * by;
-                o.x += y.x * by, o.y += y.y * by, o.z += y.z * by, o.w += y.w * by;
-            }
-            m = top;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(~0u, before, o);
+            if ((tid & 31) >= (uint32_t)o) before += x;
         }
-        finish4<BF16>(a, rq, G, cut.head, row0 + r, f, D, m, l, o, err);
+        if ((tid & 31) == 31) warp_cuts[tid >> 5] = before;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < kShareJoinThreads / 32; ++w) {
+            if (w < tid / 32) before += warp_cuts[w];
+            total += warp_cuts[w];
+        }
+        before -= cuts;
+        // one tile per CTA, unless requests have more tiles than the launch expected
+        for (uint32_t want = blockIdx.x / kChunks; want < total; want += shape.join_tiles) {
+            if (want >= before && want < before + cuts) {
+                uint32_t left = want - before;
+                for (uint32_t k = tid * kPer; k < tid * kPer + kPer; ++k)
+                    if (k < shape.row_shares && space.cuts[k].last > k && left-- == 0) found = k;
+            }
+            __syncthreads();
+            join(found);
+            __syncthreads();
+        }
     }
 }
 
@@ -680,7 +714,7 @@ namespace {
 
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kShortRows = 64;        // requests up to this many rows go to the row kernel
-constexpr uint32_t kManyPartials = 8;      // a tile cut this often is joined by many CTAs
+constexpr uint32_t kManyPartials = 8;      // shares per tile from which a tile is joined by many CTAs
 constexpr uint32_t kMinPromptGroups = 64;  // a split of a prompt: 1024 tokens or more
 
 template <int D, int NT, bool BF16, bool E4M3>
@@ -699,9 +733,9 @@ void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const 
         count_launch();
     }
     if (h.row_shares > 1) {
-        if (h.join_wide)
-            launch_pdl(kv8_rows_join_kernel<D, NT, BF16, true>, h.row_shares * 8 * NT * (D / 64), kShareJoinThreads, 0,
-                       stream, c, s, a, h, err);
+        if (h.join_tiles > 0)
+            launch_pdl(kv8_rows_join_kernel<D, NT, BF16, true>, h.join_tiles * 8 * NT * (D / 64), kShareJoinThreads, 0, stream, c,
+                       s, a, h, err);
         else
             launch_pdl(kv8_rows_join_kernel<D, NT, BF16, false>, h.row_shares, kShareJoinThreads, 0, stream, c, s, a, h, err);
         count_launch();
@@ -754,7 +788,7 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
     const uint32_t wide = h.row_tile / 8 * c.dim;
     const uint64_t wave = kSms * (wide == 512 ? 2 : c.dim == 256 || wide == 256 ? 3 : 4);
     h.row_shares = (uint32_t)std::min<uint64_t>(wave, std::max<uint64_t>(1, items * groups / kMinShare));
-    h.join_wide = h.row_shares / items >= kManyPartials;
+    h.join_tiles = items * kManyPartials <= h.row_shares ? (uint32_t)items : 0;
     h.row_floats = h.row_shares > 1 ? 2ull * h.row_shares * h.row_tile * (c.dim + 2) + 4ull * h.row_shares : 0;
     h.row_floats = ceil_div(h.row_floats, 4) * 4;   // what follows is read 16 bytes at a time
     h.prompt_rows = kv8_prompt_rows(c.dim, bf16);

@@ -9,20 +9,26 @@
 //   P = weights   TMEM -> registers -> TMEM, over the S they came from
 //   O += P V      tcgen05.mma, P from TMEM, the widened values in shared memory
 //
-// Roles (512 threads, one CTA per SM):
-//   MT warpgroups  softmax: a thread owns a row, so maxima and sums need no
-//                  exchange; two passes over its S in TMEM (maximum, weights)
-//   3 - MT         widening: pages -> registers (the loads of the next keys
-//   warpgroups     or values run while the current ones wait for their slot)
-//                  -> fp16 in the 128-byte-swizzled image the MMA reads
-//   1 warp         one thread issues the MMAs and owns TMEM
+// Roles (one CTA per SM):
+//   2 MT warpgroups  softmax: two threads share a row, half of a step's tokens
+//                    each; two passes over S in TMEM (maximum, weights), the
+//                    maxima meet in shared memory
+//   2 warpgroups     widening: pages -> registers (the loads of the next keys
+//                    or values run while the current ones wait for their slot)
+//                    -> fp16 in the 128-byte-swizzled image the MMA reads
+//   1 warp           one thread issues the MMAs and owns TMEM
+// The inner loops are kept rolled: unrolled to a row of 128 tokens in
+// registers, one thread a row, the softmax waited for instructions and took
+// 6000 cycles a step (1054 us for an 8k prompt, head dimension 128).
+// Registers move between the roles (setmaxnreg) within the launch's total:
+// UTile checks the sum.
 // With two tiles, one tile's softmax runs under the other's products; with one
 // (head dimension 256, or two-term F32 operands), S is double-buffered and the
 // next product runs under the softmax.
 //
-// The weights' token order inside a group of 16 and the values' feature order
-// inside 32 are free (both are summed or put back on output), and are chosen
-// so that a lane's value codes are 8 contiguous bytes of the image.
+// The weights' token order inside a group of 16 is free (it is summed over),
+// and is chosen so that a lane's value codes are 8 contiguous bytes of the
+// image.
 //
 // Every wait is bounded: one that gives up raises the CTA's abort flag, every
 // role leaves its loop, MMAs in flight are waited for (bounded) and TMEM is
@@ -35,25 +41,41 @@ namespace kqb {
 
 namespace {
 
-constexpr int kUThreads = 512;
 constexpr uint32_t kUTmem = 512;
+constexpr int kWidenWarps = 8;
+
+// What the roles share besides the operands, behind them in shared memory (in
+// dynamic shared memory, so that the operands begin at its start, which is
+// 1024-byte aligned: the swizzle's atoms need that).
+template <int MT>
+struct UShared {
+    uint64_t s_full[2], p_full[2], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, drained, met[MT];
+    uint32_t tmem, gave_up;
+    float meet[2][MT][2][128];   // by turn, tile, half: a row's two threads
+};
 
 template <int D, int TERMS>
 struct UTile {
     static constexpr int MT = D * TERMS <= 128 ? 2 : 1;          // query tiles of 128 rows
     static constexpr int SB = 3 - MT;                            // S buffers per tile
     static constexpr uint32_t rows = 128 * MT;
-    static constexpr uint32_t tokens = D * TERMS == 512 ? 64 : 128;   // per step
+    static constexpr uint32_t tokens = D == 256 ? 64 : 128;      // per step
     static constexpr uint32_t groups = tokens / kG;
-    static constexpr int NK = D == 256 ? 1 : 2;                  // key slots, value slots
-    static constexpr int widen_warps = 4 * (3 - MT);
+    static constexpr int NK = D * TERMS == 512 ? 1 : 2, NV = 2;  // key slots, value slots
     static constexpr uint32_t q_bytes = rows * D * 2 * TERMS;
     static constexpr uint32_t slot = tokens * D * 2;
-    static constexpr uint32_t smem = q_bytes + 2 * NK * slot + 1024;
+    static constexpr uint32_t operands = q_bytes + (NK + NV) * slot, smem = operands + sizeof(UShared<MT>);
     static constexpr uint32_t s_col = MT * D;                    // first S column
-    static constexpr int units = groups * (D / 64) / widen_warps;   // (group, 64 features) per widening warp and step
+    static constexpr int softmax_warps = 8 * MT;
+    static constexpr int threads = (softmax_warps + kWidenWarps + 4) * 32;
+    // registers a thread: what the launch gives (a multiple of 8), and the roles' shares of it
+    static constexpr int launch_regs = 65536 / threads / 8 * 8;
+    static constexpr int softmax_regs = MT == 2 ? 80 : 112, widen_regs = MT == 2 ? 64 : 96, mma_regs = 56;
+    static constexpr int units = groups * (D / 64) / kWidenWarps;   // (group, 64 features) per widening warp and step
+    static constexpr uint32_t flush = 512 / tokens;                 // steps (two-term operands)
     static_assert(s_col + MT * SB * tokens <= kUTmem, "TMEM");
-    static_assert(units * widen_warps == (int)groups * (D / 64), "units");
+    static_assert(units * kWidenWarps == (int)groups * (D / 64), "units");
+    static_assert(2 * MT * softmax_regs + 2 * widen_regs + mma_regs <= (2 * MT + 3) * launch_regs, "registers");
 };
 
 // K-major operand in 128-byte-swizzled atoms of 8 rows (1024 bytes): start
@@ -125,6 +147,34 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32
         : "memory");
 }
 
+// Two F32 values in a register pair, and packed arithmetic on them.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -137,16 +187,16 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 
 // grid (tile, head, split), the last tiles first (they see the most tokens).
 template <int D, int TERMS, bool E4M3>
-__global__ void __launch_bounds__(kUThreads, 1)
+__global__ void __launch_bounds__((UTile<D, TERMS>::threads), 1)
 kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord err) {
     using T = UTile<D, TERMS>;
-    constexpr int MT = T::MT, NK = T::NK;
+    constexpr int MT = T::MT, NK = T::NK, NV = T::NV;
     constexpr bool BF16 = TERMS == 1;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[2], p_full[2], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, drained;
-    __shared__ uint32_t tmem_slot, gave_up;
-    volatile uint32_t *quit = &gave_up;
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    UShared<MT> &sh = *reinterpret_cast<UShared<MT> *>(smem + T::operands);
+    uint64_t *const s_full = sh.s_full, *const p_full = sh.p_full, *const pv_done = sh.pv_done, *const k_full = sh.k_full,
+                    *const k_empty = sh.k_empty, *const v_full = sh.v_full, *const v_empty = sh.v_empty;
+    volatile uint32_t *quit = &sh.gave_up;
     uint8_t *k_slots = smem + T::q_bytes, *v_slots = k_slots + NK * T::slot;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t G = a.query_heads / c.heads;
@@ -154,18 +204,19 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     const uint32_t head = u % c.heads, t = shape.prompt_tiles - 1 - u / c.heads;
 
     if (tid == 0) {
-        gave_up = 0;
+        sh.gave_up = smem_u32(smem) % 1024 != 0;   // operands would be misread: give up at once
         for (int i = 0; i < 2; ++i) {
             bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], 4);
+            bar_init(&p_full[i], 8);
             bar_init(&pv_done[i], 1);
-            bar_init(&k_full[i], T::widen_warps);
+            bar_init(&k_full[i], kWidenWarps);
             bar_init(&k_empty[i], 1);
-            bar_init(&v_full[i], T::widen_warps);
+            bar_init(&v_full[i], kWidenWarps);
             bar_init(&v_empty[i], 1);
         }
-        bar_init(&q_full, 4 * MT);
-        bar_init(&drained, 1);
+        bar_init(&sh.q_full, 8 * MT);
+        for (int i = 0; i < MT; ++i) bar_init(&sh.met[i], 8);
+        bar_init(&sh.drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -186,31 +237,47 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     const int32_t *table = s.table + (uint64_t)b * s.table_stride;
     const uint32_t per_page = c.page_tokens / kG;
 
-    if (warp == 12) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+    constexpr uint32_t kMmaWarp = T::softmax_warps + kWidenWarps;
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(kUTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = sh.tmem;
 
-    if (warp < 4 * MT) {
+    if (warp < T::softmax_warps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::softmax_regs));
         // ---------------------------------------------------------- softmax
-        const uint32_t m = warp >> 2, row_in = tid & 127, row = row0 + m * 128 + row_in, token_of = row / G;
+        const uint32_t m = warp >> 3, half = warp >> 2 & 1, row_in = tid & 127, row = row0 + m * 128 + row_in, token_of = row / G;
         const bool live = row < row_end;
         const uint32_t lanes = (warp & 3) << 21;   // the warp's 32 lanes, in bits 16 and up of a TMEM address
+        // a value of the row's other thread, for this thread's: both warpgroups
+        // of the tile make the same calls (two slots, as a thread may still
+        // read the last one's)
+        uint32_t meetings = 0;
+        bool ok = true;
+        auto exchange = [&](float x) {
+            const uint32_t parity = meetings++ & 1;
+            sh.meet[parity][m][half][row_in] = x;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.met[m]);
+            ok = warp_wait(&sh.met[m], parity, quit);
+            return sh.meet[parity][m][half ^ 1][row_in];
+        };
         int32_t limit = -1;
         float factor = 0.0f;
         {
-            // this thread's row of Q, scaled and split, into the swizzled image
-            const uint64_t at = live ? (uint64_t)(rq.first + token_of) * a.q_stride + (uint64_t)(head * G + row % G) * D : 0;
+            // this thread's half row of Q, scaled and split, into the swizzled image
+            constexpr int H = D / 2;
+            const uint64_t at = live ? ((uint64_t)rq.first + token_of) * a.q_stride + (uint64_t)(head * G + row % G) * D + half * H : 0;
             float top = 0.0f;
             bool bad = false;
             if (live) {
 #pragma unroll 8
-                for (int f = 0; f < D; f += 4) {
+                for (int f = 0; f < H; f += 4) {
                     const float4 x = load4<BF16>(a.q, at + f);
                     bad |= !(fabsf(x.x) < INFINITY) || !(fabsf(x.y) < INFINITY) || !(fabsf(x.z) < INFINITY) ||
                            !(fabsf(x.w) < INFINITY);
@@ -219,18 +286,20 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 limit = (int32_t)(rq.length - rq.n + token_of);
             }
             if (bad) raise(err, kErrNonFinite);
+            top = fmaxf(top, exchange(top));
             // the largest element into [2^13, 2^14); the sign of the softmax
             // scale goes into Q, so that factors are not negative
             const int e = max((int)(__float_as_uint(top) >> 23), 27) - 127 - 13;
             const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
             factor = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll 4
-            for (int f = 0; f < D; f += 8) {
+            for (int f = 0; f < H; f += 8) {
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
                 if (live) x = load4<BF16>(a.q, at + f), y = load4<BF16>(a.q, at + f + 4);
                 x.x *= up, x.y *= up, x.z *= up, x.w *= up, y.x *= up, y.y *= up, y.z *= up, y.w *= up;
                 const uint4 h = make_uint4(pack_half(x.x, x.y), pack_half(x.z, x.w), pack_half(y.x, y.y), pack_half(y.z, y.w));
-                uint8_t *at8 = smem + m * (128 * D * 2 * TERMS) + (f / 64) * 16384 + row_in * 128 + (((f % 64 / 8) ^ (row_in & 7)) << 4);
+                const uint32_t g = half * H + f;
+                uint8_t *at8 = smem + m * (128 * D * 2 * TERMS) + (g / 64) * 16384 + row_in * 128 + (((g % 64 / 8) ^ (row_in & 7)) << 4);
                 *reinterpret_cast<uint4 *>(at8) = h;
                 if constexpr (TERMS == 2)
                     *reinterpret_cast<uint4 *>(at8 + 128 * D * 2) =
@@ -240,69 +309,115 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) bar_arrive(&q_full);
+        if (lane == 0) bar_arrive(&sh.q_full);
 
-        float mx = -INFINITY, sum = 0.0f, ref = 0.0f;
-        const uint32_t o_at = tmem + lanes + m * D;
-        bool ok = true;
-        if (m < tiles) {
-            const int32_t all_see = __reduce_min_sync(~0u, limit);   // the last token that every row of the warp sees
-            float2 sc = make_float2(0.0f, 0.0f);                     // lane l: the scales of the step's group l
-            auto fetch = [&](uint32_t j) {
-                const uint32_t g = g0 + j * T::groups + lane;
-                float2 x = make_float2(0.0f, 0.0f);
-                if (lane < T::groups && g < g1) {
-                    const int32_t id = table[g / per_page];
-                    if (id >= 0 && (uint32_t)id < c.pages)   // else: the widening warps raise the error
-                        x = *reinterpret_cast<const float2 *>(c.scales + ((uint64_t)id * c.heads + head) * 2);
+        float mx = -INFINITY, sum = 0.0f, ref = 0.0f;   // sum: of this thread's tokens
+        bool saved = false;     // sums of earlier steps are in the output (or the partials)
+        float kept = 1.0f;      // what they are to be multiplied by
+        constexpr uint32_t kHalf = T::tokens / 2;
+        const uint32_t o_at = tmem + lanes + m * D + half * (D / 2);   // this thread's half of the features
+        const bool whole = groups <= each;
+        const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, T::rows, D,
+                            (uint64_t)shape.prompt_tiles * c.heads);
+        const uint32_t in_tile = m * 128 + row_in, qh = head * G + row % G;
+        const uint64_t out_at = ((uint64_t)rq.first + token_of) * a.out_stride + (uint64_t)qh * D + half * (D / 2);
+        // O * scale + (what is saved) * keep, into the output or the partials.
+        // The accumulators' additions truncate: with two-term operands, whose
+        // result is to be good to F32, O goes out and starts anew every 512
+        // tokens (prompt chunks over 3000 tokens: error 6.5e-6 without).
+        auto move_out = [&](float scale, float keep) {
+            bool fine = true;
+#pragma unroll 1
+            for (int n = 0; n < D / 2; n += 32) {
+                uint32_t x[32];
+                if (steps > 0) {
+                    tmem_load(o_at + n, x);
+                    tmem_loaded(x);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[k] = 0;
                 }
-                return x;
+                if (!live) continue;
+                float *to = whole ? static_cast<float *>(a.out) + (BF16 ? 0 : out_at + n)
+                                  : part.o + ((uint64_t)split * T::rows + in_tile) * D + half * (D / 2) + n;
+#pragma unroll
+                for (int g = 0; g < 32; g += 4) {
+                    float4 o = make_float4(__uint_as_float(x[g]) * scale, __uint_as_float(x[g + 1]) * scale,
+                                           __uint_as_float(x[g + 2]) * scale, __uint_as_float(x[g + 3]) * scale);
+                    if (TERMS == 2 && keep != 0.0f) {
+                        const float4 y = *reinterpret_cast<const float4 *>(to + g);
+                        o.x += y.x * keep, o.y += y.y * keep, o.z += y.z * keep, o.w += y.w * keep;
+                    }
+                    fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
+                    if (BF16 && whole)
+                        store4<BF16>(a.out, out_at + n + g, o);
+                    else
+                        *reinterpret_cast<float4 *>(to + g) = o;
+                }
+            }
+            return fine;
+        };
+        if (ok && m < tiles) {
+            const int32_t all_see = __reduce_min_sync(~0u, limit);   // the last token that every row of the warp sees
+            // lane l holds the scales of the step's group l; page ids are read two steps ahead, scales one
+            auto page_of = [&](uint32_t j) {
+                const uint32_t g = g0 + j * T::groups + lane;
+                return lane < T::groups && j < steps && g < g1 ? table[g / per_page] : -1;
             };
-            float2 next = fetch(0);
+            auto scales_of = [&](int32_t id) {   // out of range: the widening warps raise the error
+                return id >= 0 && (uint32_t)id < c.pages
+                           ? *reinterpret_cast<const float2 *>(c.scales + ((uint64_t)id * c.heads + head) * 2)
+                           : make_float2(0.0f, 0.0f);
+            };
+            float2 next = scales_of(page_of(0));
+            int32_t id = page_of(1);
             for (uint32_t j = 0; j < steps; ++j) {
-                sc = next;
-                if (j + 1 < steps) next = fetch(j + 1);
+                const float2 sc = next;
+                next = scales_of(id);
+                id = page_of(j + 2);
                 const uint32_t buf = MT == 2 ? m : j & 1, phase = MT == 2 ? j & 1 : j >> 1 & 1;
-                const uint32_t s_at = tmem + lanes + T::s_col + buf * T::tokens;
-                const int32_t token = (int32_t)((g0 + j * T::groups) * kG);
-                const bool mask = token + (int32_t)T::tokens - 1 > all_see;
+                const uint32_t s_at = tmem + lanes + T::s_col + buf * T::tokens + half * kHalf;
+                const uint32_t group = half * (T::groups / 2);   // this thread's first
+                const int32_t token = (int32_t)((g0 + j * T::groups + group) * kG);
+                const bool mask = token + (int32_t)kHalf - 1 > all_see;
                 ok = warp_wait(&s_full[buf], phase, quit);
                 if (!ok) break;
                 fence_after();
                 // maximum
-                float top = -INFINITY;
+                float top = -INFINITY, most = sc.y;
 #pragma unroll
-                for (uint32_t q = 0; q < T::tokens / 32; ++q) {
+                for (int o = 1; o < (int)T::groups; o <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+                most = __shfl_sync(~0u, most, 0);
+#pragma unroll 1
+                for (uint32_t q = 0; q < kHalf / 32; ++q) {
                     uint32_t r[32];
                     tmem_load(s_at + q * 32, r);
+                    const float f0 = factor * __shfl_sync(~0u, sc.x, group + 2 * q);
+                    const float f1 = factor * __shfl_sync(~0u, sc.x, group + 2 * q + 1);
                     tmem_loaded(r);
+                    if (mask) {
+                        const int32_t seen = limit - token - (int32_t)q * 32;   // tokens 0 .. seen are visible
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float f = factor * __shfl_sync(~0u, sc.x, q * 2 + h);
-                        float x = -INFINITY;
-                        if (mask) {
-                            const int32_t first = token + (int32_t)(q * 32) + h * 16;
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                if (first + k <= limit) x = fmaxf(x, __uint_as_float(r[h * 16 + k]));
-                            x = first <= limit ? x * f : -INFINITY;
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) x = fmaxf(x, __uint_as_float(r[h * 16 + k]));
-                            x *= f;
-                        }
-                        top = fmaxf(top, x);
+                        for (int k = 0; k < 32; ++k)
+                            if (k > seen) r[k] = 0xff800000u;
                     }
-                }
-                const bool lift = top > mx + kRaise;   // -inf + 8 is -inf: the first finite logit lifts
-                float most = 0.0f;
+                    float x = -INFINITY, y = -INFINITY;
 #pragma unroll
-                for (uint32_t g = 0; g < T::groups; ++g) most = fmaxf(most, __shfl_sync(~0u, sc.y, g));
+                    for (int k = 0; k < 16; k += 2) {
+                        x = max3(x, __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+                        y = max3(y, __uint_as_float(r[16 + k]), __uint_as_float(r[17 + k]));
+                    }
+                    top = max3(top, x * f0, y * f1);   // a factor of 0 times -inf is NaN, which the maximum drops
+                }
+                top = fmaxf(top, exchange(top));
+                if (!ok) break;
+                const bool lift = top > mx + kRaise;   // -inf + 8 is -inf: the first finite logit lifts
                 float by = 1.0f;
                 if (lift) {
                     by = exp2_approx(mx - top);
                     mx = top;
                     sum *= by;
+                    kept *= by;
                 }
                 if (most > ref) {
                     // the next power of two, within the normal range
@@ -311,56 +426,84 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     by *= ref / up;
                     ref = up;
                 }
-                if (j > 0 && __any_sync(~0u, by != 1.0f)) {
-                    // O is at rest once the last step's second product is done
-                    const uint32_t last = j - 1;
-                    ok = warp_wait(&pv_done[MT == 2 ? m : 0], last & 1, quit);
+                const bool flush = TERMS == 2 && j > 0 && j % T::flush == 0;
+                // O is at rest once the last step's second product is done.  Every
+                // step waits for it before it hands its weights over, if not
+                // here: a parity wait must not fall two phases behind.
+                const bool touch = flush || (j > 0 && __any_sync(~0u, by != 1.0f));
+                if (touch) {
+                    ok = warp_wait(&pv_done[MT == 2 ? m : 0], (j - 1) & 1, quit);
                     if (!ok) break;
                     fence_after();
+                    if (flush) {
+                        // by: since the accumulators' scale; kept: since the saved sums'
+                        move_out(by * ref * (1.0f / kWeightScale), saved ? kept : 0.0f);
+                        saved = true;
+                        kept = 1.0f;
+                    } else {
 #pragma unroll 1
-                    for (int n = 0; n < D; n += 32) {
-                        uint32_t r[32];
-                        tmem_load(o_at + n, r);
-                        tmem_loaded(r);
+                        for (int n = 0; n < D / 2; n += 32) {
+                            uint32_t x[32];
+                            tmem_load(o_at + n, x);
+                            tmem_loaded(x);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * by);
-                        tmem_store32(o_at + n, r);
+                            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * by);
+                            tmem_store32(o_at + n, x);
+                        }
                     }
                 }
                 // weights
                 const float base = mx == -INFINITY ? 0.0f : mx, inv = ref > 0.0f ? kWeightScale / ref : 0.0f;
-#pragma unroll
-                for (uint32_t q = 0; q < T::tokens / 32; ++q) {
+                const uint64_t base2 = pack2(-base, -base);
+                uint64_t sum2 = 0;
+#pragma unroll 1
+                for (uint32_t q = 0; q < kHalf / 32; ++q) {
                     uint32_t r[32];
                     tmem_load(s_at + q * 32, r);
+                    float f[2], w[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        f[h] = factor * __shfl_sync(~0u, sc.x, group + 2 * q + h);
+                        w[h] = inv * __shfl_sync(~0u, sc.y, group + 2 * q + h);
+                    }
                     tmem_loaded(r);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float f = factor * __shfl_sync(~0u, sc.x, q * 2 + h);
-                        const float w = inv * __shfl_sync(~0u, sc.y, q * 2 + h);
-                        const int32_t first = token + (int32_t)(q * 32) + h * 16;
-                        float part = 0.0f;
+                        const uint64_t f2 = pack2(f[h], f[h]);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            float e = exp2_approx(fmaf(__uint_as_float(r[h * 16 + k]), f, -base));
-                            if (mask) e = first + k <= limit ? e : 0.0f;
-                            part += e;
-                            r[h * 16 + k] = __float_as_uint(e * w);
+                        for (int k = h * 16; k < h * 16 + 16; k += 2) {
+                            float x, y;
+                            unpack2(fma2(pack2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, base2), x, y);
+                            r[k] = __float_as_uint(exp2_approx(x));
+                            r[k + 1] = __float_as_uint(exp2_approx(y));
                         }
-                        sum += part;
+                    }
+                    if (mask) {
+                        const int32_t seen = limit - token - (int32_t)q * 32;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (k > seen) r[k] = 0;
                     }
                     // pairs of a group in the values' order: (0,1) (8,9) (2,3) (10,11) ...; then the low parts
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const int at = (k >> 3) * 16 + (k & 1) * 8 + (k >> 1 & 3) * 2;
-                        const float x = __uint_as_float(r[at]), y = __uint_as_float(r[at + 1]);
+                        const uint64_t e2 = pack2(__uint_as_float(r[at]), __uint_as_float(r[at + 1]));
+                        sum2 = add2(sum2, e2);
+                        float x, y;
+                        unpack2(mul2(e2, pack2(w[k >> 3], w[k >> 3])), x, y);
                         hi[k] = pack_half(x, y);
                         if constexpr (TERMS == 2) lo[k] = pack_rest(x, y, hi[k]);
                     }
                     tmem_store16(s_at + q * 32, hi);
                     if constexpr (TERMS == 2) tmem_store16(s_at + q * 32 + 16, lo);
                 }
+                float x, y;
+                unpack2(sum2, x, y);
+                sum += x + y;
+                if (j > 0 && !touch) ok = warp_wait(&pv_done[MT == 2 ? m : 0], (j - 1) & 1, quit);
+                if (!ok) break;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 fence_before();
                 __syncwarp();
@@ -368,71 +511,48 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             }
             if (ok && steps > 0) ok = warp_wait(&pv_done[MT == 2 ? m : 0], (steps - 1) & 1, quit);
             fence_after();
+            if (ok) sum += exchange(sum);
             if (ok) {
-                const bool whole = groups <= each;
-                const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, T::rows, D,
-                                    (uint64_t)shape.prompt_tiles * c.heads);
-                const uint32_t in_tile = m * 128 + row_in;
-                const float back = ref * (1.0f / kWeightScale);
-                const float scale = whole ? (sum > 0.0f ? back / sum : 0.0f) : back;
-                const uint64_t token = rq.first + token_of;
-                const uint32_t qh = head * G + row % G;
-                bool fine = sum < INFINITY;
-#pragma unroll 1
-                for (int n = 0; n < D; n += 32) {
-                    uint32_t r[32];
-                    if (steps > 0) {
-                        tmem_load(o_at + n, r);
-                        tmem_loaded(r);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) r[k] = 0;
-                    }
-                    if (!live) continue;
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) {   // column 8 i + g is feature 4 g + i
-                        const float4 o = make_float4(__uint_as_float(r[g]) * scale, __uint_as_float(r[8 + g]) * scale,
-                                                     __uint_as_float(r[16 + g]) * scale, __uint_as_float(r[24 + g]) * scale);
-                        if (whole) {
-                            fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
-                            store4<BF16>(a.out, token * a.out_stride + (uint64_t)qh * D + n + 4 * g, o);
-                        } else {
-                            *reinterpret_cast<float4 *>(part.o + ((uint64_t)split * T::rows + in_tile) * D + n + 4 * g) = o;
-                        }
-                    }
-                }
+                const float norm = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+                const bool fine = move_out(ref * (1.0f / kWeightScale) * norm, saved ? kept * norm : 0.0f);
                 if (live) {
-                    if (!whole)
-                        part.ml[in_tile * shape.prompt_splits + split] = make_float2(mx, sum);
-                    else if (a.lse != nullptr)
-                        a.lse[token * a.query_heads + qh] = sum > 0.0f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
-                    if (whole && !fine) raise(err, kErrNonFinite);
+                    if (half == 0) {
+                        if (!whole)
+                            part.ml[in_tile * shape.prompt_splits + split] = make_float2(mx, sum);
+                        else if (a.lse != nullptr)
+                            a.lse[((uint64_t)rq.first + token_of) * a.query_heads + qh] =
+                                sum > 0.0f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+                    }
+                    if (whole && (!fine || !(sum < INFINITY))) raise(err, kErrNonFinite);
                 }
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::widen_regs));
         // --------------------------------------------------------- widening
-        const uint32_t w = warp - 4 * MT;
+        const uint32_t w = warp - T::softmax_warps;
         constexpr int U = T::units;
         const uint64_t page_bytes = 2ull * c.page_tokens * D;
-        uint64_t place = 0, next = 0;   // lane l: offset of group l's codes (UINT64_MAX: behind the last)
-        auto fetch = [&](uint32_t j) {
+        // lane l: where group l's codes are (UINT64_MAX: behind the last); page ids are read two steps ahead
+        auto page_of = [&](uint32_t j) {
             const uint32_t g = g0 + j * T::groups + lane;
-            uint64_t x = UINT64_MAX;
-            if (lane < T::groups && g < g1) {
-                const int32_t id = table[g / per_page];
-                const bool in = id >= 0 && (uint32_t)id < c.pages;
-                if (!in) raise(err, kErrStep);
-                x = ((uint64_t)(in ? id : 0) * c.heads + head) * page_bytes + (uint64_t)(g % per_page) * 32 * D;
-            }
-            return x;
+            return lane < T::groups && j < steps && g < g1 ? table[g / per_page] : INT32_MIN;
         };
+        auto place_of = [&](uint32_t j, int32_t id) {
+            if (id == INT32_MIN) return UINT64_MAX;
+            const uint32_t g = g0 + j * T::groups + lane;
+            const bool in = id >= 0 && (uint32_t)id < c.pages;
+            if (!in) raise(err, kErrStep);
+            return (uint64_t)(((uint64_t)(in ? id : 0) * c.heads + head) * page_bytes + (uint64_t)(g % per_page) * 32 * D);
+        };
+        uint64_t place = place_of(0, page_of(0));
+        int32_t id = page_of(1);
         constexpr uint32_t kNothing = E4M3 ? 0u : 0x80808080u;
         // two 16-byte pieces of each of this warp's units: (group, 64 features)
         auto load = [&](uint4 (&x)[U][2], uint32_t side) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), j = unit % (D / 64);
+                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), j = unit % (D / 64);
                 const uint64_t at = __shfl_sync(~0u, place, group);
                 if (at != UINT64_MAX) {
                     const uint4 *p = reinterpret_cast<const uint4 *>(c.codes + at + side * 16 * D + j * 1024) + lane;
@@ -445,18 +565,16 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         };
         uint4 kx[U][2], vx[U][2];
         bool ok = true;
-        place = fetch(0);
         if (steps > 0) load(kx, 0);
         for (uint32_t j = 0; j < steps; ++j) {
-            const uint32_t slot = j % NK;
-            if (j + 1 < steps) next = fetch(j + 1);
+            const uint32_t slot = j % NK, vslot = j % NV;
             load(vx, 1);
             if (j >= (uint32_t)NK) ok = warp_wait(&k_empty[slot], (j / NK - 1) & 1, quit);
             if (!ok) break;
             // keys: piece h is token 8 h + g, features 16 t .. + 15: two 16-byte chunks of its row
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), f = unit % (D / 64);
+                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), f = unit % (D / 64);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t r = group * 16 + h * 8 + (lane >> 2), t2 = (lane & 3) * 2;
@@ -473,16 +591,17 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&k_full[slot]);
-            place = next;
+            place = place_of(j + 1, id);
+            id = page_of(j + 2);
             if (j + 1 < steps) load(kx, 0);
-            if (j >= (uint32_t)NK) ok = warp_wait(&v_empty[slot], (j / NK - 1) & 1, quit);
+            if (j >= (uint32_t)NV) ok = warp_wait(&v_empty[vslot], (j / NV - 1) & 1, quit);
             if (!ok) break;
-            // values: word i of piece h is feature 32 h + 4 g + i, tokens 2t, 2t + 1, 2t + 8, 2t + 9: row
-            // 8 i + g of the feature block's 32, bytes 8 t of the group's 32
+            // values: word i of piece h is feature 32 h + 4 g + i (a row of the image), tokens 2t, 2t + 1,
+            // 2t + 8, 2t + 9: bytes 8 t of the group's 32
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), f = unit % (D / 64);
-                uint8_t *block = v_slots + slot * T::slot + (group >> 2) * (D * 128);
+                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), f = unit % (D / 64);
+                uint8_t *block = v_slots + vslot * T::slot + (group >> 2) * (D * 128);
                 const uint32_t chunk = (group & 3) * 2 + (lane >> 1 & 1), half = (lane & 1) * 8;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -491,16 +610,19 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     for (int i = 0; i < 4; ++i) {
                         uint2 x;
                         widen<E4M3>(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w, x.x, x.y);
-                        const uint32_t n = f * 64 + h * 32 + i * 8 + (lane >> 2);
+                        const uint32_t n = f * 64 + h * 32 + (lane >> 2) * 4 + i;
                         *reinterpret_cast<uint2 *>(block + n * 128 + ((chunk ^ (n & 7)) << 4) + half) = x;
                     }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) bar_arrive(&v_full[slot]);
+            if (lane == 0) bar_arrive(&v_full[vslot]);
         }
-    } else if (warp == 12 && lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::mma_regs));
+    }
+    if (warp == kMmaWarp && lane == 0) {
         // ------------------------------------------------------------- MMAs
         const uint32_t q_at = smem_u32(smem), k_at = smem_u32(k_slots), v_at = smem_u32(v_slots);
         auto first_product = [&](uint32_t m, uint32_t buf, uint32_t slot) {
@@ -526,7 +648,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     umma_ts<D>(d, p + k / 2 * 32 + term * 16 + k % 2 * 8, vb, !(fresh && k == 0 && term == TERMS - 1));
             }
         };
-        bool ok = bar_wait(&q_full, 0, quit);
+        bool ok = bar_wait(&sh.q_full, 0, quit);
         if (ok && steps > 0) {
             ok = bar_wait(&k_full[0], 0, quit);
             if (ok) {
@@ -539,13 +661,14 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             }
             for (uint32_t j = 0; ok && j < steps; ++j) {
                 const bool more = j + 1 < steps;
-                const uint32_t slot = j % NK, slot1 = (j + 1) % NK;
+                const uint32_t slot = j % NV, slot1 = (j + 1) % NK;
+                const bool fresh = j == 0 || (TERMS == 2 && j % T::flush == 0);
                 if constexpr (MT == 2) {
                     for (uint32_t m = 0; ok && m < tiles; ++m) {
-                        ok = bar_wait(&p_full[m], j & 1, quit) && (m > 0 || bar_wait(&v_full[slot], j / NK & 1, quit));
+                        ok = bar_wait(&p_full[m], j & 1, quit) && (m > 0 || bar_wait(&v_full[slot], j / NV & 1, quit));
                         if (!ok) break;
                         fence_after();
-                        second_product(m, m, slot, j == 0);
+                        second_product(m, m, slot, fresh);
                         umma_commit(&pv_done[m]);
                         if (m + 1 == tiles) umma_commit(&v_empty[slot]);
                         if (more) {
@@ -570,24 +693,24 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                         umma_commit(&s_full[(j + 1) & 1]);
                         umma_commit(&k_empty[slot1]);
                     }
-                    ok = bar_wait(&p_full[j & 1], j >> 1 & 1, quit) && bar_wait(&v_full[slot], j / NK & 1, quit);
+                    ok = bar_wait(&p_full[j & 1], j >> 1 & 1, quit) && bar_wait(&v_full[slot], j / NV & 1, quit);
                     if (!ok) break;
                     fence_after();
-                    second_product(0, j & 1, slot, j == 0);
+                    second_product(0, j & 1, slot, fresh);
                     umma_commit(&pv_done[0]);
                     umma_commit(&v_empty[slot]);
                 }
             }
         }
         // nothing of this CTA's is in flight after this
-        umma_commit(&drained);
-        bar_wait(&drained, 0);
-        if (*quit) raise(err, kErrTimeout);
+        umma_commit(&sh.drained);
+        bar_wait(&sh.drained, 0, quit);
     }
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (tid == 0 && *quit) raise(err, kErrTimeout);
+    if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kUTmem));
     }
@@ -604,7 +727,7 @@ void launch_prompt(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, cons
         cudaFuncSetAttribute(kv8_prompt_kernel<D, TERMS, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
     KernelTimer timer("kv8_prompt", stream);
-    launch_pdl(kv8_prompt_kernel<D, TERMS, E4M3>, h.prompt_tiles * c.heads * h.prompt_splits, kUThreads, smem, stream, c, s, a, h,
+    launch_pdl(kv8_prompt_kernel<D, TERMS, E4M3>, h.prompt_tiles * c.heads * h.prompt_splits, UTile<D, TERMS>::threads, smem, stream, c, s, a, h,
                err);
     count_launch();
 }
