@@ -80,6 +80,15 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
     return false;
 }
 
+// The same for a whole warp, with the same answer in every lane; one lane
+// polls (polls are shared-memory traffic: with all lanes the row kernel took
+// 203 us for 64 F32 sequences, not 192).
+__device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, volatile uint32_t *quit = nullptr) {
+    uint32_t ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = bar_wait(bar, parity, quit);
+    return __shfl_sync(~0u, ok, 0) != 0;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

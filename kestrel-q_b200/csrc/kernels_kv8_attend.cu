@@ -445,7 +445,7 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
                 fetch(i + 32, 1);
             }
             const uint32_t slot = (used + i) % ST;
-            ok = bar_wait(&full[warp][slot], (used + i) / ST & 1u);
+            ok = bar_wait_warp(&full[warp][slot], (used + i) / ST & 1u);
             if (!ok) break;
             const float ks = __shfl_sync(~0u, scales[0].x, i & 31), vs = __shfl_sync(~0u, scales[0].y, i & 31);
             const uint32_t token = (g0 + warp + i * kRowWarps) * kG;
@@ -460,7 +460,7 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
         if (!ok) {
             // a wait gave up: let the other copies land before the CTA exits
             if (lane == 0) raise(err, kErrTimeout);
-            for (uint32_t k = i; k < issued; ++k) bar_wait(&full[warp][(used + k) % ST], (used + k) / ST & 1u);
+            for (uint32_t k = i; k < issued; ++k) bar_wait_warp(&full[warp][(used + k) % ST], (used + k) / ST & 1u);
         }
         used += mine;
 

@@ -3,28 +3,29 @@
 // kernels_kv8_attend.cu.)
 //
 // One CTA takes MT tiles of 128 query rows (request rows r = token * G + head)
-// of one key/value head and walks the tokens they see, 128 (or 64) at a time:
+// of one key/value head and walks the tokens they see, 64 at a time:
 //
 //   S = Q K^T     tcgen05.mma, Q and the widened keys in shared memory
-//   P = weights   TMEM -> registers -> TMEM, over the S they came from
+//   P = weights   TMEM -> registers -> TMEM
 //   O += P V      tcgen05.mma, P from TMEM, the widened values in shared memory
 //
 // Roles (one CTA per SM):
-//   2 MT warpgroups  softmax: two threads share a row, half of a step's tokens
-//                    each; two passes over S in TMEM (maximum, weights), the
-//                    maxima meet in shared memory
-//   2 warpgroups     widening: pages -> registers (the loads of the next keys
-//                    or values run while the current ones wait for their slot)
-//                    -> fp16 in the 128-byte-swizzled image the MMA reads
-//   1 warp           one thread issues the MMAs and owns TMEM
-// The inner loops are kept rolled: unrolled to a row of 128 tokens in
-// registers, one thread a row, the softmax waited for instructions and took
-// 6000 cycles a step (1054 us for an 8k prompt, head dimension 128).
+//   MT warpgroups      softmax: a thread owns a row (its 64 S values sit in
+//                      registers), so maxima and sums need no exchange
+//   1 or 2 warpgroups  widening: pages -> registers (the loads of the next
+//                      keys or values run while the current ones wait for
+//                      their slot) -> fp16 in the 128-byte-swizzled image the
+//                      MMA reads
+//   1 warp             one thread issues the MMAs and owns TMEM
+// S is free again as soon as the softmax has it in registers, and the weights
+// have two buffers of their own: the next step's first product runs under this
+// step's softmax, and a row's chain is its softmax alone. (With the weights over
+// the S they came from, the next product had to wait for the second one: 4600
+// cycles for 64 tokens, 1118 us for an 8k prompt at head dimension 128.)
+// Loads bypass L1: the operands leave it a few KB, and allocating there took
+// bandwidth from the MMA's operands (64-row products at 250 cycles, not 48).
 // Registers move between the roles (setmaxnreg) within the launch's total:
 // UTile checks the sum.
-// With two tiles, one tile's softmax runs under the other's products; with one
-// (head dimension 256, or two-term F32 operands), S is double-buffered and the
-// next product runs under the softmax.
 //
 // The weights' token order inside a group of 16 is free (it is summed over),
 // and is chosen so that a lane's value codes are 8 contiguous bytes of the
@@ -42,40 +43,41 @@ namespace kqb {
 namespace {
 
 constexpr uint32_t kUTmem = 512;
-constexpr int kWidenWarps = 8;
 
 // What the roles share besides the operands, behind them in shared memory (in
 // dynamic shared memory, so that the operands begin at its start, which is
 // 1024-byte aligned: the swizzle's atoms need that).
-template <int MT>
 struct UShared {
-    uint64_t s_full[2], p_full[2], pv_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full, drained, met[MT];
+    uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];   // by tile
+    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], q_full, drained, back[2];
     uint32_t tmem, gave_up;
-    float meet[2][MT][2][128];   // by turn, tile, half: a row's two threads
 };
 
 template <int D, int TERMS>
 struct UTile {
     static constexpr int MT = D * TERMS <= 128 ? 2 : 1;          // query tiles of 128 rows
-    static constexpr int SB = 3 - MT;                            // S buffers per tile
     static constexpr uint32_t rows = 128 * MT;
-    static constexpr uint32_t tokens = D == 256 ? 64 : 128;      // per step
+    static constexpr uint32_t tokens = 64;                       // per step
     static constexpr uint32_t groups = tokens / kG;
-    static constexpr int NK = D * TERMS == 512 ? 1 : 2, NV = 2;  // key slots, value slots
+    static constexpr int NK = D * TERMS == 512 ? 1 : D == 256 ? 2 : 3, NV = D * TERMS == 512 ? 2 : 3;   // key and value slots
     static constexpr uint32_t q_bytes = rows * D * 2 * TERMS;
     static constexpr uint32_t slot = tokens * D * 2;
-    static constexpr uint32_t operands = q_bytes + (NK + NV) * slot, smem = operands + sizeof(UShared<MT>);
-    static constexpr uint32_t s_col = MT * D;                    // first S column
-    static constexpr int softmax_warps = 8 * MT;
-    static constexpr int threads = (softmax_warps + kWidenWarps + 4) * 32;
+    static constexpr uint32_t operands = q_bytes + (NK + NV) * slot, smem = operands + sizeof(UShared);
+    // TMEM columns: O of each tile, then per tile S and two buffers of weights
+    // (32 columns a term)
+    static constexpr uint32_t s_col = MT * D, p_cols = tokens / 2 * TERMS, tile_cols = tokens + 2 * p_cols;
+    static constexpr int softmax_warps = 4 * MT, widen_warps = D == 64 ? 4 : 8;
+    static constexpr int threads = (softmax_warps + widen_warps + 4) * 32;
     // registers a thread: what the launch gives (a multiple of 8), and the roles' shares of it
-    static constexpr int launch_regs = 65536 / threads / 8 * 8;
-    static constexpr int softmax_regs = MT == 2 ? 80 : 112, widen_regs = MT == 2 ? 64 : 96, mma_regs = 56;
-    static constexpr int units = groups * (D / 64) / kWidenWarps;   // (group, 64 features) per widening warp and step
+    static constexpr int launch_regs = 65536 / threads / 8 * 8 < 168 ? 65536 / threads / 8 * 8 : 168;
+    static constexpr int softmax_regs = threads == 640 ? 136 : 168, widen_regs = threads == 640 ? 80 : 104;
+    static constexpr int mma_regs = threads == 640 ? 48 : 56;
+    static constexpr int units = groups * (D / 64) / widen_warps;   // (group, 64 features) per widening warp and step
     static constexpr uint32_t flush = 512 / tokens;                 // steps (two-term operands)
-    static_assert(s_col + MT * SB * tokens <= kUTmem, "TMEM");
-    static_assert(units * kWidenWarps == (int)groups * (D / 64), "units");
-    static_assert(2 * MT * softmax_regs + 2 * widen_regs + mma_regs <= (2 * MT + 3) * launch_regs, "registers");
+    static_assert(s_col + MT * tile_cols <= kUTmem, "TMEM");
+    static_assert(units * widen_warps == (int)groups * (D / 64), "units");
+    static_assert(MT * softmax_regs + widen_warps / 4 * widen_regs + mma_regs <= threads / 128 * launch_regs, "registers");
+    static_assert(smem <= 227 * 1024, "shared memory");
 };
 
 // K-major operand in 128-byte-swizzled atoms of 8 rows (1024 bytes): start
@@ -178,11 +180,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// A bounded wait of a whole warp: the same answer in every lane.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *quit) {
-    return __all_sync(~0u, bar_wait(bar, parity, quit));
-}
-
 }  // namespace
 
 // grid (tile, head, split), the last tiles first (they see the most tokens).
@@ -193,9 +190,9 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     constexpr int MT = T::MT, NK = T::NK, NV = T::NV;
     constexpr bool BF16 = TERMS == 1;
     extern __shared__ __align__(1024) uint8_t smem[];
-    UShared<MT> &sh = *reinterpret_cast<UShared<MT> *>(smem + T::operands);
-    uint64_t *const s_full = sh.s_full, *const p_full = sh.p_full, *const pv_done = sh.pv_done, *const k_full = sh.k_full,
-                    *const k_empty = sh.k_empty, *const v_full = sh.v_full, *const v_empty = sh.v_empty;
+    UShared &sh = *reinterpret_cast<UShared *>(smem + T::operands);
+    uint64_t *const pv_done = sh.pv_done, *const k_full = sh.k_full, *const k_empty = sh.k_empty, *const v_full = sh.v_full,
+                    *const v_empty = sh.v_empty;
     volatile uint32_t *quit = &sh.gave_up;
     uint8_t *k_slots = smem + T::q_bytes, *v_slots = k_slots + NK * T::slot;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -205,17 +202,20 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
 
     if (tid == 0) {
         sh.gave_up = smem_u32(smem) % 1024 != 0;   // operands would be misread: give up at once
-        for (int i = 0; i < 2; ++i) {
-            bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], 8);
-            bar_init(&pv_done[i], 1);
-            bar_init(&k_full[i], kWidenWarps);
+        for (int m = 0; m < 2; ++m) {
+            bar_init(&pv_done[m], 1);
+            bar_init(&sh.back[m], 4);
+            bar_init(&sh.s_full[m], 1);
+            bar_init(&sh.s_free[m], 4);
+            bar_init(&sh.p_full[m], 4);
+        }
+        for (int i = 0; i < 3; ++i) {
+            bar_init(&k_full[i], T::widen_warps);
             bar_init(&k_empty[i], 1);
-            bar_init(&v_full[i], kWidenWarps);
+            bar_init(&v_full[i], T::widen_warps);
             bar_init(&v_empty[i], 1);
         }
-        bar_init(&sh.q_full, 8 * MT);
-        for (int i = 0; i < MT; ++i) bar_init(&sh.met[i], 8);
+        bar_init(&sh.q_full, 4 * MT);
         bar_init(&sh.drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -237,7 +237,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     const int32_t *table = s.table + (uint64_t)b * s.table_stride;
     const uint32_t per_page = c.page_tokens / kG;
 
-    constexpr uint32_t kMmaWarp = T::softmax_warps + kWidenWarps;
+    constexpr uint32_t kMmaWarp = T::softmax_warps + T::widen_warps;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(kUTmem));
@@ -251,33 +251,19 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     if (warp < T::softmax_warps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::softmax_regs));
         // ---------------------------------------------------------- softmax
-        const uint32_t m = warp >> 3, half = warp >> 2 & 1, row_in = tid & 127, row = row0 + m * 128 + row_in, token_of = row / G;
+        const uint32_t m = warp >> 2, row_in = tid & 127, row = row0 + m * 128 + row_in, token_of = row / G;
         const bool live = row < row_end;
         const uint32_t lanes = (warp & 3) << 21;   // the warp's 32 lanes, in bits 16 and up of a TMEM address
-        // a value of the row's other thread, for this thread's: both warpgroups
-        // of the tile make the same calls (two slots, as a thread may still
-        // read the last one's)
-        uint32_t meetings = 0;
-        bool ok = true;
-        auto exchange = [&](float x) {
-            const uint32_t parity = meetings++ & 1;
-            sh.meet[parity][m][half][row_in] = x;
-            __syncwarp();
-            if (lane == 0) bar_arrive(&sh.met[m]);
-            ok = warp_wait(&sh.met[m], parity, quit);
-            return sh.meet[parity][m][half ^ 1][row_in];
-        };
         int32_t limit = -1;
         float factor = 0.0f;
         {
-            // this thread's half row of Q, scaled and split, into the swizzled image
-            constexpr int H = D / 2;
-            const uint64_t at = live ? ((uint64_t)rq.first + token_of) * a.q_stride + (uint64_t)(head * G + row % G) * D + half * H : 0;
+            // this thread's row of Q, scaled and split, into the swizzled image
+            const uint64_t at = live ? ((uint64_t)rq.first + token_of) * a.q_stride + (uint64_t)(head * G + row % G) * D : 0;
             float top = 0.0f;
             bool bad = false;
             if (live) {
-#pragma unroll 8
-                for (int f = 0; f < H; f += 4) {
+#pragma unroll 16
+                for (int f = 0; f < D; f += 4) {
                     const float4 x = load4<BF16>(a.q, at + f);
                     bad |= !(fabsf(x.x) < INFINITY) || !(fabsf(x.y) < INFINITY) || !(fabsf(x.z) < INFINITY) ||
                            !(fabsf(x.w) < INFINITY);
@@ -286,20 +272,18 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 limit = (int32_t)(rq.length - rq.n + token_of);
             }
             if (bad) raise(err, kErrNonFinite);
-            top = fmaxf(top, exchange(top));
             // the largest element into [2^13, 2^14); the sign of the softmax
             // scale goes into Q, so that factors are not negative
             const int e = max((int)(__float_as_uint(top) >> 23), 27) - 127 - 13;
             const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), a.scale_log2);
             factor = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll 4
-            for (int f = 0; f < H; f += 8) {
+#pragma unroll 8
+            for (int f = 0; f < D; f += 8) {
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
                 if (live) x = load4<BF16>(a.q, at + f), y = load4<BF16>(a.q, at + f + 4);
                 x.x *= up, x.y *= up, x.z *= up, x.w *= up, y.x *= up, y.y *= up, y.z *= up, y.w *= up;
                 const uint4 h = make_uint4(pack_half(x.x, x.y), pack_half(x.z, x.w), pack_half(y.x, y.y), pack_half(y.z, y.w));
-                const uint32_t g = half * H + f;
-                uint8_t *at8 = smem + m * (128 * D * 2 * TERMS) + (g / 64) * 16384 + row_in * 128 + (((g % 64 / 8) ^ (row_in & 7)) << 4);
+                uint8_t *at8 = smem + m * (128 * D * 2 * TERMS) + (f / 64) * 16384 + row_in * 128 + (((f % 64 / 8) ^ (row_in & 7)) << 4);
                 *reinterpret_cast<uint4 *>(at8) = h;
                 if constexpr (TERMS == 2)
                     *reinterpret_cast<uint4 *>(at8 + 128 * D * 2) =
@@ -311,53 +295,72 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.q_full);
 
-        float mx = -INFINITY, sum = 0.0f, ref = 0.0f;   // sum: of this thread's tokens
-        bool saved = false;     // sums of earlier steps are in the output (or the partials)
-        float kept = 1.0f;      // what they are to be multiplied by
-        constexpr uint32_t kHalf = T::tokens / 2;
-        const uint32_t o_at = tmem + lanes + m * D + half * (D / 2);   // this thread's half of the features
+        float mx = -INFINITY, sum = 0.0f, ref = 0.0f;
+        const uint32_t o_at = tmem + lanes + m * D;
         const bool whole = groups <= each;
         const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, T::rows, D,
                             (uint64_t)shape.prompt_tiles * c.heads);
-        const uint32_t in_tile = m * 128 + row_in, qh = head * G + row % G;
-        const uint64_t out_at = ((uint64_t)rq.first + token_of) * a.out_stride + (uint64_t)qh * D + half * (D / 2);
-        // O * scale + (what is saved) * keep, into the output or the partials.
-        // The accumulators' additions truncate: with two-term operands, whose
-        // result is to be good to F32, O goes out and starts anew every 512
-        // tokens (prompt chunks over 3000 tokens: error 6.5e-6 without).
-        auto move_out = [&](float scale, float keep) {
-            bool fine = true;
-#pragma unroll 1
-            for (int n = 0; n < D / 2; n += 32) {
-                uint32_t x[32];
-                if (steps > 0) {
-                    tmem_load(o_at + n, x);
-                    tmem_loaded(x);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = 0;
-                }
-                if (!live) continue;
-                float *to = whole ? static_cast<float *>(a.out) + (BF16 ? 0 : out_at + n)
-                                  : part.o + ((uint64_t)split * T::rows + in_tile) * D + half * (D / 2) + n;
-#pragma unroll
-                for (int g = 0; g < 32; g += 4) {
-                    float4 o = make_float4(__uint_as_float(x[g]) * scale, __uint_as_float(x[g + 1]) * scale,
-                                           __uint_as_float(x[g + 2]) * scale, __uint_as_float(x[g + 3]) * scale);
-                    if (TERMS == 2 && keep != 0.0f) {
-                        const float4 y = *reinterpret_cast<const float4 *>(to + g);
-                        o.x += y.x * keep, o.y += y.y * keep, o.z += y.z * keep, o.w += y.w * keep;
-                    }
-                    fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
-                    if (BF16 && whole)
-                        store4<BF16>(a.out, out_at + n + g, o);
-                    else
-                        *reinterpret_cast<float4 *>(to + g) = o;
-                }
-            }
-            return fine;
+        const uint32_t in_tile = m * 128 + row_in;
+        // where row r of this tile goes
+        auto row_out = [&](uint32_t r) {
+            return whole ? ((uint64_t)rq.first + r / G) * a.out_stride + (uint64_t)(head * G + r % G) * D
+                         : (uint64_t)split * T::rows * D + (uint64_t)(r - row0) * D;
         };
-        if (ok && m < tiles) {
+        float *const out32 = whole ? static_cast<float *>(a.out) : part.o;
+        // Sums of earlier steps (TERMS == 2).  The accumulators' additions
+        // truncate; with two-term operands, whose result is to be good to F32,
+        // O goes out and starts anew every 512 tokens (prompt chunks over 3000
+        // tokens: error 6.5e-6 without, 1.5e-6 with).  It goes to the tile's own
+        // output rows (or partials), as long as they are not final: where all
+        // 128 rows exist, value 4 f .. 4 f + 3 of row r is the (128 f + r)-th 16
+        // bytes of the rows one after another, so that a warp writes 512
+        // contiguous bytes; in a tile's rest, in its row.
+        bool saved = false;
+        float kept = 1.0f;      // what the saved sums are to be multiplied by
+        const bool full_tile = row0 + m * 128 + 128 <= row_end;
+        auto save = [&](float scale, float keep, bool final_to_tmem) {
+            constexpr uint32_t Q = D / 4, kRowsOn = 128 / Q;   // pieces in a row; rows from piece f to piece f + 1 of a thread
+            const uint32_t first = row0 + m * 128 + row_in / Q;
+            float *to = out32 + (full_tile ? row_out(first) + row_in % Q * 4 : row_out(row));
+            uint32_t in_group = first % G;
+            const int64_t wrap = whole ? (int64_t)a.out_stride - (int64_t)G * D : 0;
+#pragma unroll 1
+            for (int n = 0; n < D; n += 32) {
+                uint32_t x[32];
+                float *at[8];
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    at[g] = to;
+                    if (full_tile) {
+                        to += kRowsOn * D;
+                        for (in_group += kRowsOn; in_group >= G; in_group -= G) to += wrap;
+                    } else {
+                        to += 4;
+                    }
+                }
+                tmem_load(o_at + n, x);
+                float4 y[8];
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    y[g] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (keep != 0.0f && live) y[g] = __ldcg(reinterpret_cast<const float4 *>(at[g]));
+                }
+                tmem_loaded(x);
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const float4 o = make_float4(__uint_as_float(x[4 * g]) * scale + y[g].x * keep,
+                                                 __uint_as_float(x[4 * g + 1]) * scale + y[g].y * keep,
+                                                 __uint_as_float(x[4 * g + 2]) * scale + y[g].z * keep,
+                                                 __uint_as_float(x[4 * g + 3]) * scale + y[g].w * keep);
+                    x[4 * g] = __float_as_uint(o.x), x[4 * g + 1] = __float_as_uint(o.y);
+                    x[4 * g + 2] = __float_as_uint(o.z), x[4 * g + 3] = __float_as_uint(o.w);
+                    if (!final_to_tmem && live) __stcg(reinterpret_cast<float4 *>(at[g]), o);
+                }
+                if (final_to_tmem) tmem_store32(o_at + n, x);
+            }
+        };
+        bool ok = true;
+        if (m < tiles) {
             const int32_t all_see = __reduce_min_sync(~0u, limit);   // the last token that every row of the warp sees
             // lane l holds the scales of the step's group l; page ids are read two steps ahead, scales one
             auto page_of = [&](uint32_t j) {
@@ -371,49 +374,56 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             };
             float2 next = scales_of(page_of(0));
             int32_t id = page_of(1);
+#pragma unroll 1
             for (uint32_t j = 0; j < steps; ++j) {
                 const float2 sc = next;
                 next = scales_of(id);
                 id = page_of(j + 2);
-                const uint32_t buf = MT == 2 ? m : j & 1, phase = MT == 2 ? j & 1 : j >> 1 & 1;
-                const uint32_t s_at = tmem + lanes + T::s_col + buf * T::tokens + half * kHalf;
-                const uint32_t group = half * (T::groups / 2);   // this thread's first
-                const int32_t token = (int32_t)((g0 + j * T::groups + group) * kG);
-                const bool mask = token + (int32_t)kHalf - 1 > all_see;
-                ok = warp_wait(&s_full[buf], phase, quit);
+                const uint32_t s_at = tmem + lanes + T::s_col + m * T::tile_cols, p_at = s_at + T::tokens + (j & 1) * T::p_cols;
+                const int32_t token = (int32_t)((g0 + j * T::groups) * kG);
+                float f[T::groups], w[T::groups], most = 0.0f;
+#pragma unroll
+                for (uint32_t g = 0; g < T::groups; ++g) {
+                    f[g] = factor * __shfl_sync(~0u, sc.x, g);
+                    w[g] = __shfl_sync(~0u, sc.y, g);
+                    most = fmaxf(most, w[g]);
+                }
+                ok = bar_wait_warp(&sh.s_full[m], j & 1, quit);
                 if (!ok) break;
                 fence_after();
-                // maximum
-                float top = -INFINITY, most = sc.y;
+                uint32_t r[2][32];
+                tmem_load(s_at, r[0]);
+                tmem_load(s_at + 32, r[1]);
+                tmem_loaded(r[0]);
+                tmem_loaded(r[1]);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.s_free[m]);
+                if (token + (int32_t)T::tokens - 1 > all_see) {
+                    const int32_t seen = limit - token;   // tokens 0 .. seen are visible
 #pragma unroll
-                for (int o = 1; o < (int)T::groups; o <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
-                most = __shfl_sync(~0u, most, 0);
-#pragma unroll 1
-                for (uint32_t q = 0; q < kHalf / 32; ++q) {
-                    uint32_t r[32];
-                    tmem_load(s_at + q * 32, r);
-                    const float f0 = factor * __shfl_sync(~0u, sc.x, group + 2 * q);
-                    const float f1 = factor * __shfl_sync(~0u, sc.x, group + 2 * q + 1);
-                    tmem_loaded(r);
-                    if (mask) {
-                        const int32_t seen = limit - token - (int32_t)q * 32;   // tokens 0 .. seen are visible
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (k > seen) r[k] = 0xff800000u;
-                    }
-                    float x = -INFINITY, y = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        x = max3(x, __uint_as_float(r[k]), __uint_as_float(r[k + 1]));
-                        y = max3(y, __uint_as_float(r[16 + k]), __uint_as_float(r[17 + k]));
-                    }
-                    top = max3(top, x * f0, y * f1);   // a factor of 0 times -inf is NaN, which the maximum drops
+                    for (int k = 0; k < 64; ++k)
+                        if (k > seen) r[k / 32][k % 32] = 0xff800000u;
                 }
-                top = fmaxf(top, exchange(top));
-                if (!ok) break;
-                const bool lift = top > mx + kRaise;   // -inf + 8 is -inf: the first finite logit lifts
+                float top = -INFINITY;
+                {
+                    float x[T::groups];
+#pragma unroll
+                    for (uint32_t g = 0; g < T::groups; ++g) x[g] = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2)
+#pragma unroll
+                        for (uint32_t g = 0; g < T::groups; ++g)
+                            x[g] = max3(x[g], __uint_as_float(r[g / 2][g % 2 * 16 + k]), __uint_as_float(r[g / 2][g % 2 * 16 + k + 1]));
+#pragma unroll
+                    for (uint32_t g = 0; g < T::groups; ++g) {
+                        // a factor of 0 (a zero page) would make -inf NaN
+                        if (f[g] == 0.0f) f[g] = 1.0e-38f;
+                        top = fmaxf(top, x[g] * f[g]);
+                    }
+                }
                 float by = 1.0f;
-                if (lift) {
+                if (top > mx + kRaise) {   // -inf + 8 is -inf: the first finite logit lifts
                     by = exp2_approx(mx - top);
                     mx = top;
                     sum *= by;
@@ -429,20 +439,21 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 const bool flush = TERMS == 2 && j > 0 && j % T::flush == 0;
                 // O is at rest once the last step's second product is done.  Every
                 // step waits for it before it hands its weights over, if not
-                // here: a parity wait must not fall two phases behind.
+                // here: a parity wait must not fall two phases behind, and the
+                // buffer that these weights go into is free since the last wait.
                 const bool touch = flush || (j > 0 && __any_sync(~0u, by != 1.0f));
                 if (touch) {
-                    ok = warp_wait(&pv_done[MT == 2 ? m : 0], (j - 1) & 1, quit);
+                    ok = bar_wait_warp(&pv_done[m], (j - 1) & 1, quit);
                     if (!ok) break;
                     fence_after();
                     if (flush) {
                         // by: since the accumulators' scale; kept: since the saved sums'
-                        move_out(by * ref * (1.0f / kWeightScale), saved ? kept : 0.0f);
+                        if constexpr (TERMS == 2) save(by * ref * (1.0f / kWeightScale), saved ? kept : 0.0f, false);
                         saved = true;
                         kept = 1.0f;
                     } else {
 #pragma unroll 1
-                        for (int n = 0; n < D / 2; n += 32) {
+                        for (int n = 0; n < D; n += 32) {
                             uint32_t x[32];
                             tmem_load(o_at + n, x);
                             tmem_loaded(x);
@@ -455,75 +466,91 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 // weights
                 const float base = mx == -INFINITY ? 0.0f : mx, inv = ref > 0.0f ? kWeightScale / ref : 0.0f;
                 const uint64_t base2 = pack2(-base, -base);
-                uint64_t sum2 = 0;
-#pragma unroll 1
-                for (uint32_t q = 0; q < kHalf / 32; ++q) {
-                    uint32_t r[32];
-                    tmem_load(s_at + q * 32, r);
-                    float f[2], w[2];
+                uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                for (uint32_t q = 0; q < 2; ++q) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        f[h] = factor * __shfl_sync(~0u, sc.x, group + 2 * q + h);
-                        w[h] = inv * __shfl_sync(~0u, sc.y, group + 2 * q + h);
-                    }
-                    tmem_loaded(r);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint64_t f2 = pack2(f[h], f[h]);
+                        const uint64_t f2 = pack2(f[2 * q + h], f[2 * q + h]);
 #pragma unroll
                         for (int k = h * 16; k < h * 16 + 16; k += 2) {
                             float x, y;
-                            unpack2(fma2(pack2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, base2), x, y);
-                            r[k] = __float_as_uint(exp2_approx(x));
-                            r[k + 1] = __float_as_uint(exp2_approx(y));
+                            unpack2(fma2(pack2(__uint_as_float(r[q][k]), __uint_as_float(r[q][k + 1])), f2, base2), x, y);
+                            r[q][k] = __float_as_uint(exp2_approx(x));
+                            r[q][k + 1] = __float_as_uint(exp2_approx(y));
                         }
-                    }
-                    if (mask) {
-                        const int32_t seen = limit - token - (int32_t)q * 32;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (k > seen) r[k] = 0;
                     }
                     // pairs of a group in the values' order: (0,1) (8,9) (2,3) (10,11) ...; then the low parts
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const int at = (k >> 3) * 16 + (k & 1) * 8 + (k >> 1 & 3) * 2;
-                        const uint64_t e2 = pack2(__uint_as_float(r[at]), __uint_as_float(r[at + 1]));
-                        sum2 = add2(sum2, e2);
+                        const uint64_t e2 = pack2(__uint_as_float(r[q][at]), __uint_as_float(r[q][at + 1]));
+                        sum2[k & 1] = add2(sum2[k & 1], e2);
+                        const float v = w[2 * q + (k >> 3)] * inv;
                         float x, y;
-                        unpack2(mul2(e2, pack2(w[k >> 3], w[k >> 3])), x, y);
+                        unpack2(mul2(e2, pack2(v, v)), x, y);
                         hi[k] = pack_half(x, y);
                         if constexpr (TERMS == 2) lo[k] = pack_rest(x, y, hi[k]);
                     }
-                    tmem_store16(s_at + q * 32, hi);
-                    if constexpr (TERMS == 2) tmem_store16(s_at + q * 32 + 16, lo);
+                    tmem_store16(p_at + q * 16, hi);
+                    if constexpr (TERMS == 2) tmem_store16(p_at + 32 + q * 16, lo);
                 }
                 float x, y;
-                unpack2(sum2, x, y);
+                unpack2(add2(sum2[0], sum2[1]), x, y);
                 sum += x + y;
-                if (j > 0 && !touch) ok = warp_wait(&pv_done[MT == 2 ? m : 0], (j - 1) & 1, quit);
+                if (j > 0 && !touch) ok = bar_wait_warp(&pv_done[m], (j - 1) & 1, quit);
                 if (!ok) break;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&p_full[buf]);
+                if (lane == 0) bar_arrive(&sh.p_full[m]);
             }
-            if (ok && steps > 0) ok = warp_wait(&pv_done[MT == 2 ? m : 0], (steps - 1) & 1, quit);
+            if (ok && steps > 0) ok = bar_wait_warp(&pv_done[m], (steps - 1) & 1, quit);
             fence_after();
-            if (ok) sum += exchange(sum);
+            float scale = ref * (1.0f / kWeightScale);
+            if (TERMS == 2 && ok && saved) {
+                // the saved sums come back into TMEM before any row is final
+                save(scale, kept, true);
+                scale = 1.0f;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.back[m]);
+                ok = bar_wait_warp(&sh.back[m], 0, quit);
+            }
             if (ok) {
-                const float norm = whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
-                const bool fine = move_out(ref * (1.0f / kWeightScale) * norm, saved ? kept * norm : 0.0f);
-                if (live) {
-                    if (half == 0) {
-                        if (!whole)
-                            part.ml[in_tile * shape.prompt_splits + split] = make_float2(mx, sum);
-                        else if (a.lse != nullptr)
-                            a.lse[((uint64_t)rq.first + token_of) * a.query_heads + qh] =
-                                sum > 0.0f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+                if (whole) scale *= sum > 0.0f ? 1.0f / sum : 0.0f;
+                bool fine = sum < INFINITY;
+                const uint64_t to = row_out(row);
+#pragma unroll 1
+                for (int n = 0; n < D; n += 32) {
+                    uint32_t x[32];
+                    if (steps > 0) {
+                        tmem_load(o_at + n, x);
+                        tmem_loaded(x);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) x[k] = 0;
                     }
-                    if (whole && (!fine || !(sum < INFINITY))) raise(err, kErrNonFinite);
+                    if (!live) continue;
+#pragma unroll
+                    for (int g = 0; g < 32; g += 4) {
+                        const float4 o = make_float4(__uint_as_float(x[g]) * scale, __uint_as_float(x[g + 1]) * scale,
+                                                     __uint_as_float(x[g + 2]) * scale, __uint_as_float(x[g + 3]) * scale);
+                        fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
+                        if (whole)
+                            store4<BF16>(a.out, to + n + g, o);
+                        else
+                            *reinterpret_cast<float4 *>(out32 + to + n + g) = o;
+                    }
+                }
+                if (live) {
+                    if (!whole)
+                        part.ml[in_tile * shape.prompt_splits + split] = make_float2(mx, sum);
+                    else if (a.lse != nullptr)
+                        a.lse[((uint64_t)rq.first + token_of) * a.query_heads + head * G + row % G] =
+                            sum > 0.0f ? (mx + log2f(sum)) * kLn2 : -INFINITY;
+                    if (whole && !fine) raise(err, kErrNonFinite);
                 }
             }
         }
@@ -552,12 +579,12 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         auto load = [&](uint4 (&x)[U][2], uint32_t side) {
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), j = unit % (D / 64);
+                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), j = unit % (D / 64);
                 const uint64_t at = __shfl_sync(~0u, place, group);
                 if (at != UINT64_MAX) {
                     const uint4 *p = reinterpret_cast<const uint4 *>(c.codes + at + side * 16 * D + j * 1024) + lane;
-                    x[k][0] = __ldg(p);
-                    x[k][1] = __ldg(p + 32);
+                    x[k][0] = __ldcg(p);
+                    x[k][1] = __ldcg(p + 32);
                 } else {
                     x[k][0] = x[k][1] = make_uint4(kNothing, kNothing, kNothing, kNothing);
                 }
@@ -569,12 +596,12 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         for (uint32_t j = 0; j < steps; ++j) {
             const uint32_t slot = j % NK, vslot = j % NV;
             load(vx, 1);
-            if (j >= (uint32_t)NK) ok = warp_wait(&k_empty[slot], (j / NK - 1) & 1, quit);
+            if (j >= (uint32_t)NK) ok = bar_wait_warp(&k_empty[slot], (j / NK - 1) & 1, quit);
             if (!ok) break;
             // keys: piece h is token 8 h + g, features 16 t .. + 15: two 16-byte chunks of its row
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), f = unit % (D / 64);
+                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), f = unit % (D / 64);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t r = group * 16 + h * 8 + (lane >> 2), t2 = (lane & 3) * 2;
@@ -594,13 +621,13 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             place = place_of(j + 1, id);
             id = page_of(j + 2);
             if (j + 1 < steps) load(kx, 0);
-            if (j >= (uint32_t)NV) ok = warp_wait(&v_empty[vslot], (j / NV - 1) & 1, quit);
+            if (j >= (uint32_t)NV) ok = bar_wait_warp(&v_empty[vslot], (j / NV - 1) & 1, quit);
             if (!ok) break;
             // values: word i of piece h is feature 32 h + 4 g + i (a row of the image), tokens 2t, 2t + 1,
             // 2t + 8, 2t + 9: bytes 8 t of the group's 32
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                const uint32_t unit = w + k * kWidenWarps, group = unit / (D / 64), f = unit % (D / 64);
+                const uint32_t unit = w + k * T::widen_warps, group = unit / (D / 64), f = unit % (D / 64);
                 uint8_t *block = v_slots + vslot * T::slot + (group >> 2) * (D * 128);
                 const uint32_t chunk = (group & 3) * 2 + (lane >> 1 & 1), half = (lane & 1) * 8;
 #pragma unroll
@@ -625,8 +652,8 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     if (warp == kMmaWarp && lane == 0) {
         // ------------------------------------------------------------- MMAs
         const uint32_t q_at = smem_u32(smem), k_at = smem_u32(k_slots), v_at = smem_u32(v_slots);
-        auto first_product = [&](uint32_t m, uint32_t buf, uint32_t slot) {
-            const uint32_t d = tmem + T::s_col + buf * T::tokens;
+        auto first_product = [&](uint32_t m, uint32_t slot) {
+            const uint32_t d = tmem + T::s_col + m * T::tile_cols;
 #pragma unroll
             for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
@@ -639,67 +666,40 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 }
         };
         auto second_product = [&](uint32_t m, uint32_t buf, uint32_t slot, bool fresh) {
-            const uint32_t p = tmem + T::s_col + buf * T::tokens, d = tmem + m * D;
+            const uint32_t p = tmem + T::s_col + m * T::tile_cols + T::tokens + buf * T::p_cols, d = tmem + m * D;
+            const uint64_t vb = operand(v_at + slot * T::slot);
 #pragma unroll
-            for (uint32_t k = 0; k < T::tokens / 16; ++k) {
-                const uint64_t vb = operand(v_at + slot * T::slot + (k / 4) * (D * 128)) + 2 * (k % 4);
+            for (uint32_t k = 0; k < T::tokens / 16; ++k)
 #pragma unroll
                 for (int term = TERMS - 1; term >= 0; --term)
-                    umma_ts<D>(d, p + k / 2 * 32 + term * 16 + k % 2 * 8, vb, !(fresh && k == 0 && term == TERMS - 1));
-            }
+                    umma_ts<D>(d, p + term * 32 + k * 8, vb + 2 * k, !(fresh && k == 0 && term == TERMS - 1));
         };
         bool ok = bar_wait(&sh.q_full, 0, quit);
-        if (ok && steps > 0) {
-            ok = bar_wait(&k_full[0], 0, quit);
-            if (ok) {
-                fence_after();
-                for (uint32_t m = 0; m < tiles; ++m) {
-                    first_product(m, MT == 2 ? m : 0, 0);
-                    umma_commit(&s_full[MT == 2 ? m : 0]);
-                }
-                umma_commit(&k_empty[0]);
-            }
-            for (uint32_t j = 0; ok && j < steps; ++j) {
-                const bool more = j + 1 < steps;
-                const uint32_t slot = j % NV, slot1 = (j + 1) % NK;
-                const bool fresh = j == 0 || (TERMS == 2 && j % T::flush == 0);
-                if constexpr (MT == 2) {
-                    for (uint32_t m = 0; ok && m < tiles; ++m) {
-                        ok = bar_wait(&p_full[m], j & 1, quit) && (m > 0 || bar_wait(&v_full[slot], j / NV & 1, quit));
-                        if (!ok) break;
-                        fence_after();
-                        second_product(m, m, slot, fresh);
-                        umma_commit(&pv_done[m]);
-                        if (m + 1 == tiles) umma_commit(&v_empty[slot]);
-                        if (more) {
-                            // the next S overwrites the weights that the product reads
-                            ok = (m > 0 || bar_wait(&k_full[slot1], (j + 1) / NK & 1, quit)) &&
-                                 bar_wait(&pv_done[m], j & 1, quit);
-                            if (!ok) break;
-                            fence_after();
-                            first_product(m, m, slot1);
-                            umma_commit(&s_full[m]);
-                            if (m + 1 == tiles) umma_commit(&k_empty[slot1]);
-                        }
-                    }
-                } else {
-                    if (more) {
-                        // into the buffer whose weights the last step's product read
-                        ok = bar_wait(&k_full[slot1], (j + 1) / NK & 1, quit) &&
-                             (j == 0 || bar_wait(&pv_done[0], (j - 1) & 1, quit));
-                        if (!ok) break;
-                        fence_after();
-                        first_product(0, (j + 1) & 1, slot1);
-                        umma_commit(&s_full[(j + 1) & 1]);
-                        umma_commit(&k_empty[slot1]);
-                    }
-                    ok = bar_wait(&p_full[j & 1], j >> 1 & 1, quit) && bar_wait(&v_full[slot], j / NV & 1, quit);
+        for (uint32_t j = 0; ok && j <= steps; ++j) {
+            // the first products of step j, once the softmax holds step j - 1's
+            if (j < steps) {
+                ok = bar_wait(&k_full[j % NK], j / NK & 1, quit);
+                for (uint32_t m = 0; ok && m < tiles; ++m) {
+                    if (j > 0) ok = bar_wait(&sh.s_free[m], (j - 1) & 1, quit);
                     if (!ok) break;
                     fence_after();
-                    second_product(0, j & 1, slot, fresh);
-                    umma_commit(&pv_done[0]);
-                    umma_commit(&v_empty[slot]);
+                    first_product(m, j % NK);
+                    umma_commit(&sh.s_full[m]);
                 }
+                umma_commit(&k_empty[j % NK]);
+            }
+            // the second products of step j - 1
+            if (ok && j > 0) {
+                const uint32_t i = j - 1;
+                ok = bar_wait(&v_full[i % NV], i / NV & 1, quit);
+                for (uint32_t m = 0; ok && m < tiles; ++m) {
+                    ok = bar_wait(&sh.p_full[m], i & 1, quit);
+                    if (!ok) break;
+                    fence_after();
+                    second_product(m, i & 1, i % NV, i == 0 || (TERMS == 2 && i % T::flush == 0));
+                    umma_commit(&pv_done[m]);
+                }
+                umma_commit(&v_empty[i % NV]);
             }
         }
         // nothing of this CTA's is in flight after this
