@@ -15,7 +15,7 @@ constexpr uint32_t kG = kKv8GroupTokens;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kRaise = 8.0f;        // a logit this far above m raises it
 constexpr float kWeightScale = 64.0f; // 2^6
-constexpr uint32_t kWaitPolls = 1u << 26;
+constexpr uint32_t kTryNs = 100000;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kPromptUnit = 8;   // groups: a prompt's split is whole steps of 128 tokens
 
@@ -54,22 +54,23 @@ __device__ __forceinline__ uint64_t global_ns() {
 }
 
 // Bounded wait for the phase of `bar` with the given parity: gives up after
-// kWaitPolls polls or kWaitNs, or (quit not null) once *quit is set, and sets
-// it then.
+// kWaitNs, or (quit not null) once *quit is set, and sets it then.  Each try
+// may suspend the thread for up to kTryNs: a warp that polls takes issue slots
+// from the others of its scheduler.
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *quit = nullptr) {
-    const uint32_t a = smem_u32(bar);
     uint64_t t0 = 0;   // the clock is read only once a wait is slow
-    for (uint32_t i = 0; i < kWaitPolls; ++i) {
+#pragma unroll 1
+    for (uint32_t i = 0;; ++i) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.b32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
-            : "r"(a), "r"(parity)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(kTryNs)
             : "memory");
         if (done) return true;
-        if ((i & 63) == 63) {
+        if ((i & 15) == 15) {
             if (quit != nullptr && *quit) return false;
             const uint64_t now = global_ns();
             if (t0 == 0) t0 = now;

@@ -401,6 +401,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 if (lane == 0) bar_arrive(&sh.s_free[m]);
                 if (token + (int32_t)T::tokens - 1 > all_see) {
                     const int32_t seen = limit - token;   // tokens 0 .. seen are visible
+                    asm volatile("");   // a branch, not 128 instructions that every step executes under a predicate
 #pragma unroll
                     for (int k = 0; k < 64; ++k)
                         if (k > seen) r[k / 32][k % 32] = 0xff800000u;
@@ -592,11 +593,12 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         };
         uint4 kx[U][2], vx[U][2];
         bool ok = true;
+        uint32_t slot = 0, k_phase = 1, vslot = 0, v_phase = 1;   // a slot's first wait is for no phase: it is free
         if (steps > 0) load(kx, 0);
+#pragma unroll 1
         for (uint32_t j = 0; j < steps; ++j) {
-            const uint32_t slot = j % NK, vslot = j % NV;
             load(vx, 1);
-            if (j >= (uint32_t)NK) ok = bar_wait_warp(&k_empty[slot], (j / NK - 1) & 1, quit);
+            if (j >= (uint32_t)NK) ok = bar_wait_warp(&k_empty[slot], k_phase, quit);
             if (!ok) break;
             // keys: piece h is token 8 h + g, features 16 t .. + 15: two 16-byte chunks of its row
 #pragma unroll
@@ -618,10 +620,11 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&k_full[slot]);
+            if (++slot == NK) slot = 0, k_phase ^= 1;
             place = place_of(j + 1, id);
             id = page_of(j + 2);
             if (j + 1 < steps) load(kx, 0);
-            if (j >= (uint32_t)NV) ok = bar_wait_warp(&v_empty[vslot], (j / NV - 1) & 1, quit);
+            if (j >= (uint32_t)NV) ok = bar_wait_warp(&v_empty[vslot], v_phase, quit);
             if (!ok) break;
             // values: word i of piece h is feature 32 h + 4 g + i (a row of the image), tokens 2t, 2t + 1,
             // 2t + 8, 2t + 9: bytes 8 t of the group's 32
@@ -645,6 +648,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&v_full[vslot]);
+            if (++vslot == NV) vslot = 0, v_phase ^= 1;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::mma_regs));
@@ -654,16 +658,15 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         const uint32_t q_at = smem_u32(smem), k_at = smem_u32(k_slots), v_at = smem_u32(v_slots);
         auto first_product = [&](uint32_t m, uint32_t slot) {
             const uint32_t d = tmem + T::s_col + m * T::tile_cols;
+            const uint64_t qa = operand(q_at + m * (128 * D * 2 * TERMS)), kb = operand(k_at + slot * T::slot);
 #pragma unroll
             for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
-                for (int f = 0; f < D / 64; ++f) {
-                    const uint64_t qa = operand(q_at + m * (128 * D * 2 * TERMS) + term * (128 * D * 2) + f * 16384);
-                    const uint64_t kb = operand(k_at + slot * T::slot + f * (T::tokens * 128));
+                for (int f = 0; f < D / 64; ++f)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_ss<T::tokens>(d, qa + 2 * k, kb + 2 * k, !(term == TERMS - 1 && f == 0 && k == 0));
-                }
+                    for (int k = 0; k < 4; ++k)   // descriptors count 16 bytes
+                        umma_ss<T::tokens>(d, qa + term * (128 * D / 8) + f * 1024 + 2 * k, kb + f * (T::tokens * 8) + 2 * k,
+                                           !(term == TERMS - 1 && f == 0 && k == 0));
         };
         auto second_product = [&](uint32_t m, uint32_t buf, uint32_t slot, bool fresh) {
             const uint32_t p = tmem + T::s_col + m * T::tile_cols + T::tokens + buf * T::p_cols, d = tmem + m * D;
@@ -675,31 +678,37 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     umma_ts<D>(d, p + term * 32 + k * 8, vb + 2 * k, !(fresh && k == 0 && term == TERMS - 1));
         };
         bool ok = bar_wait(&sh.q_full, 0, quit);
+        uint32_t k_slot = 0, k_phase = 0, v_slot = 0, v_phase = 0;
+#pragma unroll 1
         for (uint32_t j = 0; ok && j <= steps; ++j) {
             // the first products of step j, once the softmax holds step j - 1's
             if (j < steps) {
-                ok = bar_wait(&k_full[j % NK], j / NK & 1, quit);
+                ok = bar_wait(&k_full[k_slot], k_phase, quit);
+#pragma unroll 1
                 for (uint32_t m = 0; ok && m < tiles; ++m) {
                     if (j > 0) ok = bar_wait(&sh.s_free[m], (j - 1) & 1, quit);
                     if (!ok) break;
                     fence_after();
-                    first_product(m, j % NK);
+                    first_product(m, k_slot);
                     umma_commit(&sh.s_full[m]);
                 }
-                umma_commit(&k_empty[j % NK]);
+                umma_commit(&k_empty[k_slot]);
+                if (++k_slot == NK) k_slot = 0, k_phase ^= 1;
             }
             // the second products of step j - 1
             if (ok && j > 0) {
                 const uint32_t i = j - 1;
-                ok = bar_wait(&v_full[i % NV], i / NV & 1, quit);
+                ok = bar_wait(&v_full[v_slot], v_phase, quit);
+#pragma unroll 1
                 for (uint32_t m = 0; ok && m < tiles; ++m) {
                     ok = bar_wait(&sh.p_full[m], i & 1, quit);
                     if (!ok) break;
                     fence_after();
-                    second_product(m, i & 1, i % NV, i == 0 || (TERMS == 2 && i % T::flush == 0));
+                    second_product(m, i & 1, v_slot, i == 0 || (TERMS == 2 && i % T::flush == 0));
                     umma_commit(&pv_done[m]);
                 }
-                umma_commit(&v_empty[i % NV]);
+                umma_commit(&v_empty[v_slot]);
+                if (++v_slot == NV) v_slot = 0, v_phase ^= 1;
             }
         }
         // nothing of this CTA's is in flight after this
