@@ -656,26 +656,40 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     if (warp == kMmaWarp && lane == 0) {
         // ------------------------------------------------------------- MMAs
         const uint32_t q_at = smem_u32(smem), k_at = smem_u32(k_slots), v_at = smem_u32(v_slots);
+        // Rolled loops: this thread's instructions are fetched anew every step,
+        // and unrolled they took longer than the products (descriptors count 16
+        // bytes).
+        const uint64_t q_desc = operand(q_at), k_desc = operand(k_at), v_desc = operand(v_at);
         auto first_product = [&](uint32_t m, uint32_t slot) {
             const uint32_t d = tmem + T::s_col + m * T::tile_cols;
-            const uint64_t qa = operand(q_at + m * (128 * D * 2 * TERMS)), kb = operand(k_at + slot * T::slot);
-#pragma unroll
-            for (int term = TERMS - 1; term >= 0; --term)
-#pragma unroll
-                for (int f = 0; f < D / 64; ++f)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)   // descriptors count 16 bytes
-                        umma_ss<T::tokens>(d, qa + term * (128 * D / 8) + f * 1024 + 2 * k, kb + f * (T::tokens * 8) + 2 * k,
-                                           !(term == TERMS - 1 && f == 0 && k == 0));
+            uint64_t qa = q_desc + m * (128 * D * TERMS / 8);
+            uint32_t more = 0;
+#pragma unroll 1
+            for (int term = 0; term < TERMS; ++term) {
+                uint64_t kb = k_desc + slot * (T::slot / 16);
+#pragma unroll 1
+                for (int f = 0; f < D / 64; ++f, qa += 1024, kb += T::tokens * 8) {
+                    umma_ss<T::tokens>(d, qa, kb, more);
+                    umma_ss<T::tokens>(d, qa + 2, kb + 2, 1);
+                    umma_ss<T::tokens>(d, qa + 4, kb + 4, 1);
+                    umma_ss<T::tokens>(d, qa + 6, kb + 6, 1);
+                    more = 1;
+                }
+            }
         };
         auto second_product = [&](uint32_t m, uint32_t buf, uint32_t slot, bool fresh) {
-            const uint32_t p = tmem + T::s_col + m * T::tile_cols + T::tokens + buf * T::p_cols, d = tmem + m * D;
-            const uint64_t vb = operand(v_at + slot * T::slot);
-#pragma unroll
-            for (uint32_t k = 0; k < T::tokens / 16; ++k)
-#pragma unroll
-                for (int term = TERMS - 1; term >= 0; --term)
-                    umma_ts<D>(d, p + term * 32 + k * 8, vb + 2 * k, !(fresh && k == 0 && term == TERMS - 1));
+            uint32_t p = tmem + T::s_col + m * T::tile_cols + T::tokens + buf * T::p_cols;
+            const uint32_t d = tmem + m * D;
+            uint32_t more = !fresh;
+#pragma unroll 1
+            for (int term = 0; term < TERMS; ++term, p += 32) {
+                const uint64_t vb = v_desc + slot * (T::slot / 16);
+                umma_ts<D>(d, p, vb, more);
+                umma_ts<D>(d, p + 8, vb + 2, 1);
+                umma_ts<D>(d, p + 16, vb + 4, 1);
+                umma_ts<D>(d, p + 24, vb + 6, 1);
+                more = 1;
+            }
         };
         bool ok = bar_wait(&sh.q_full, 0, quit);
         uint32_t k_slot = 0, k_phase = 0, v_slot = 0, v_phase = 0;
