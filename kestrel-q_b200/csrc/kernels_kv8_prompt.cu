@@ -3,25 +3,20 @@
 // kernels_kv8_attend.cu.)
 //
 // One CTA takes MT tiles of 128 query rows (request rows r = token * G + head)
-// of one key/value head and walks the tokens they see, 64 at a time:
+// of one key/value head and walks the tokens they see, 128 or 64 at a time:
 //
 //   S = Q K^T     tcgen05.mma, Q and the widened keys in shared memory
 //   P = weights   TMEM -> registers -> TMEM
 //   O += P V      tcgen05.mma, P from TMEM, the widened values in shared memory
 //
 // Roles (one CTA per SM):
-//   MT warpgroups      softmax: a thread owns a row (its 64 S values sit in
+//   MT warpgroups      softmax: a thread owns a row (a step's S sits in its
 //                      registers), so maxima and sums need no exchange
-//   1 or 2 warpgroups  widening: pages -> registers (the loads of the next
+//   3 - MT warpgroups  widening: pages -> registers (the loads of the next
 //                      keys or values run while the current ones wait for
 //                      their slot) -> fp16 in the 128-byte-swizzled image the
 //                      MMA reads
 //   1 warp             one thread issues the MMAs and owns TMEM
-// S is free again as soon as the softmax has it in registers, and the weights
-// have two buffers of their own: the next step's first product runs under this
-// step's softmax, and a row's chain is its softmax alone. (With the weights over
-// the S they came from, the next product had to wait for the second one: 4600
-// cycles for 64 tokens, 1118 us for an 8k prompt at head dimension 128.)
 // Loads bypass L1: the operands leave it a few KB, and allocating there took
 // bandwidth from the MMA's operands (64-row products at 250 cycles, not 48).
 // Registers move between the roles (setmaxnreg) within the launch's total:
@@ -57,25 +52,29 @@ template <int D, int TERMS>
 struct UTile {
     static constexpr int MT = D * TERMS <= 128 ? 2 : 1;          // query tiles of 128 rows
     static constexpr uint32_t rows = 128 * MT;
-    static constexpr uint32_t tokens = 64;                       // per step
+    // Two tiles: 128 tokens a step, the weights over the S they came from; one
+    // tile's softmax runs under the other's products.  One tile: 64 tokens a
+    // step, the weights in two buffers of their own, so that S is free as soon
+    // as it is in registers and the next product runs under the softmax.
+    static constexpr bool alias = MT == 2;
+    static constexpr uint32_t tokens = alias ? 128 : 64;         // per step
     static constexpr uint32_t groups = tokens / kG;
-    static constexpr int NK = D * TERMS == 512 ? 1 : D == 256 ? 2 : 3, NV = D * TERMS == 512 ? 2 : 3;   // key and value slots
+    static constexpr int NK = D * TERMS == 512 ? 1 : D == 256 || alias ? 2 : 3;   // key and value slots
+    static constexpr int NV = D * TERMS == 512 || alias ? 2 : 3;
     static constexpr uint32_t q_bytes = rows * D * 2 * TERMS;
     static constexpr uint32_t slot = tokens * D * 2;
     static constexpr uint32_t operands = q_bytes + (NK + NV) * slot, smem = operands + sizeof(UShared);
-    // TMEM columns: O of each tile, then per tile S and two buffers of weights
-    // (32 columns a term)
-    static constexpr uint32_t s_col = MT * D, p_cols = tokens / 2 * TERMS, tile_cols = tokens + 2 * p_cols;
-    static constexpr int softmax_warps = 4 * MT, widen_warps = D == 64 ? 4 : 8;
-    static constexpr int threads = (softmax_warps + widen_warps + 4) * 32;
-    // registers a thread: what the launch gives (a multiple of 8), and the roles' shares of it
-    static constexpr int launch_regs = 65536 / threads / 8 * 8 < 168 ? 65536 / threads / 8 * 8 : 168;
-    static constexpr int softmax_regs = threads == 640 ? 136 : 168, widen_regs = threads == 640 ? 80 : 104;
-    static constexpr int mma_regs = threads == 640 ? 48 : 56;
+    // TMEM columns: O of each tile, then per tile S and the weights (tokens / 2
+    // columns a term)
+    static constexpr uint32_t s_col = MT * D, p_cols = tokens / 2 * TERMS, tile_cols = alias ? tokens : tokens + 2 * p_cols;
+    static constexpr int softmax_warps = 4 * MT, widen_warps = 4 * (3 - MT);
+    static constexpr int threads = 512, launch_regs = 128;
+    static constexpr int softmax_regs = MT == 2 ? 184 : 168, widen_regs = MT == 2 ? 96 : 104, mma_regs = 48;
     static constexpr int units = groups * (D / 64) / widen_warps;   // (group, 64 features) per widening warp and step
     static constexpr uint32_t flush = 512 / tokens;                 // steps (two-term operands)
     static_assert(s_col + MT * tile_cols <= kUTmem, "TMEM");
     static_assert(units * widen_warps == (int)groups * (D / 64), "units");
+    static_assert(softmax_warps + widen_warps + 4 == threads / 32 && p_cols <= (alias ? tokens : 2 * tokens), "roles");
     static_assert(MT * softmax_regs + widen_warps / 4 * widen_regs + mma_regs <= threads / 128 * launch_regs, "registers");
     static_assert(smem <= 227 * 1024, "shared memory");
 };
@@ -379,7 +378,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 const float2 sc = next;
                 next = scales_of(id);
                 id = page_of(j + 2);
-                const uint32_t s_at = tmem + lanes + T::s_col + m * T::tile_cols, p_at = s_at + T::tokens + (j & 1) * T::p_cols;
+                const uint32_t s_at = tmem + lanes + T::s_col + m * T::tile_cols, p_at = T::alias ? s_at : s_at + T::tokens + (j & 1) * T::p_cols;
                 const int32_t token = (int32_t)((g0 + j * T::groups) * kG);
                 float f[T::groups], w[T::groups], most = 0.0f;
 #pragma unroll
@@ -391,19 +390,21 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 ok = bar_wait_warp(&sh.s_full[m], j & 1, quit);
                 if (!ok) break;
                 fence_after();
-                uint32_t r[2][32];
-                tmem_load(s_at, r[0]);
-                tmem_load(s_at + 32, r[1]);
-                tmem_loaded(r[0]);
-                tmem_loaded(r[1]);
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&sh.s_free[m]);
+                uint32_t r[T::tokens / 32][32];
+#pragma unroll
+                for (uint32_t q = 0; q < T::tokens / 32; ++q) tmem_load(s_at + q * 32, r[q]);
+#pragma unroll
+                for (uint32_t q = 0; q < T::tokens / 32; ++q) tmem_loaded(r[q]);
+                if constexpr (!T::alias) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh.s_free[m]);
+                }
                 if (token + (int32_t)T::tokens - 1 > all_see) {
                     const int32_t seen = limit - token;   // tokens 0 .. seen are visible
-                    asm volatile("");   // a branch, not 128 instructions that every step executes under a predicate
+                    asm volatile("");   // a branch, not instructions that every step executes under a predicate
 #pragma unroll
-                    for (int k = 0; k < 64; ++k)
+                    for (int k = 0; k < (int)T::tokens; ++k)
                         if (k > seen) r[k / 32][k % 32] = 0xff800000u;
                 }
                 float top = -INFINITY;
@@ -469,7 +470,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 const uint64_t base2 = pack2(-base, -base);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
-                for (uint32_t q = 0; q < 2; ++q) {
+                for (uint32_t q = 0; q < T::tokens / 32; ++q) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint64_t f2 = pack2(f[2 * q + h], f[2 * q + h]);
@@ -495,7 +496,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                         if constexpr (TERMS == 2) lo[k] = pack_rest(x, y, hi[k]);
                     }
                     tmem_store16(p_at + q * 16, hi);
-                    if constexpr (TERMS == 2) tmem_store16(p_at + 32 + q * 16, lo);
+                    if constexpr (TERMS == 2) tmem_store16(p_at + T::tokens / 2 + q * 16, lo);
                 }
                 float x, y;
                 unpack2(add2(sum2[0], sum2[1]), x, y);
@@ -662,10 +663,11 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         const uint64_t q_desc = operand(q_at), k_desc = operand(k_at), v_desc = operand(v_at);
         auto first_product = [&](uint32_t m, uint32_t slot) {
             const uint32_t d = tmem + T::s_col + m * T::tile_cols;
-            uint64_t qa = q_desc + m * (128 * D * TERMS / 8);
             uint32_t more = 0;
+            // low parts first: on a sum that is still small, additions that truncate lose little
 #pragma unroll 1
-            for (int term = 0; term < TERMS; ++term) {
+            for (int term = TERMS - 1; term >= 0; --term) {
+                uint64_t qa = q_desc + (m * TERMS + term) * (128 * D / 8);
                 uint64_t kb = k_desc + slot * (T::slot / 16);
 #pragma unroll 1
                 for (int f = 0; f < D / 64; ++f, qa += 1024, kb += T::tokens * 8) {
@@ -678,51 +680,77 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             }
         };
         auto second_product = [&](uint32_t m, uint32_t buf, uint32_t slot, bool fresh) {
-            uint32_t p = tmem + T::s_col + m * T::tile_cols + T::tokens + buf * T::p_cols;
             const uint32_t d = tmem + m * D;
             uint32_t more = !fresh;
 #pragma unroll 1
-            for (int term = 0; term < TERMS; ++term, p += 32) {
-                const uint64_t vb = v_desc + slot * (T::slot / 16);
-                umma_ts<D>(d, p, vb, more);
-                umma_ts<D>(d, p + 8, vb + 2, 1);
-                umma_ts<D>(d, p + 16, vb + 4, 1);
-                umma_ts<D>(d, p + 24, vb + 6, 1);
-                more = 1;
+            for (int term = TERMS - 1; term >= 0; --term) {
+                uint32_t p = tmem + T::s_col + m * T::tile_cols + (T::alias ? 0 : T::tokens + buf * T::p_cols) + term * (T::tokens / 2);
+                uint64_t vb = v_desc + slot * (T::slot / 16);
+#pragma unroll 1
+                for (uint32_t block = 0; block < T::tokens / 64; ++block, p += 32, vb += D * 8) {
+                    umma_ts<D>(d, p, vb, more);
+                    umma_ts<D>(d, p + 8, vb + 2, 1);
+                    umma_ts<D>(d, p + 16, vb + 4, 1);
+                    umma_ts<D>(d, p + 24, vb + 6, 1);
+                    more = 1;
+                }
             }
         };
         bool ok = bar_wait(&sh.q_full, 0, quit);
         uint32_t k_slot = 0, k_phase = 0, v_slot = 0, v_phase = 0;
+        auto next_k = [&] {
+            umma_commit(&k_empty[k_slot]);
+            if (++k_slot == NK) k_slot = 0, k_phase ^= 1;
+        };
+        auto next_v = [&] {
+            umma_commit(&v_empty[v_slot]);
+            if (++v_slot == NV) v_slot = 0, v_phase ^= 1;
+        };
 #pragma unroll 1
         for (uint32_t j = 0; ok && j <= steps; ++j) {
-            // the first products of step j, once the softmax holds step j - 1's
-            if (j < steps) {
-                ok = bar_wait(&k_full[k_slot], k_phase, quit);
+            const uint32_t i = j - 1;
+            const bool fresh = i == 0 || (TERMS == 2 && i % T::flush == 0);
+            if constexpr (T::alias) {
+                // tile by tile: the second product of step j - 1, then the first
+                // of step j over the weights that it read
 #pragma unroll 1
-                for (uint32_t m = 0; ok && m < tiles; ++m) {
-                    if (j > 0) ok = bar_wait(&sh.s_free[m], (j - 1) & 1, quit);
+                for (uint32_t m = 0; m < tiles; ++m) {
+                    if (j > 0) {
+                        ok = (m > 0 || bar_wait(&v_full[v_slot], v_phase, quit)) && bar_wait(&sh.p_full[m], i & 1, quit);
+                        if (!ok) break;
+                        fence_after();
+                        second_product(m, 0, v_slot, fresh);
+                        umma_commit(&pv_done[m]);
+                    }
+                    if (j < steps) {
+                        ok = (m > 0 || bar_wait(&k_full[k_slot], k_phase, quit)) && (j == 0 || bar_wait(&pv_done[m], i & 1, quit));
+                        if (!ok) break;
+                        fence_after();
+                        first_product(m, k_slot);
+                        umma_commit(&sh.s_full[m]);
+                    }
+                }
+                if (j > 0) next_v();
+                if (j < steps) next_k();
+            } else {
+                // the first product of step j, once the softmax holds step j - 1's
+                if (j < steps) {
+                    ok = bar_wait(&k_full[k_slot], k_phase, quit) && (j == 0 || bar_wait(&sh.s_free[0], i & 1, quit));
                     if (!ok) break;
                     fence_after();
-                    first_product(m, k_slot);
-                    umma_commit(&sh.s_full[m]);
+                    first_product(0, k_slot);
+                    umma_commit(&sh.s_full[0]);
+                    next_k();
                 }
-                umma_commit(&k_empty[k_slot]);
-                if (++k_slot == NK) k_slot = 0, k_phase ^= 1;
-            }
-            // the second products of step j - 1
-            if (ok && j > 0) {
-                const uint32_t i = j - 1;
-                ok = bar_wait(&v_full[v_slot], v_phase, quit);
-#pragma unroll 1
-                for (uint32_t m = 0; ok && m < tiles; ++m) {
-                    ok = bar_wait(&sh.p_full[m], i & 1, quit);
+                // the second product of step j - 1
+                if (j > 0) {
+                    ok = bar_wait(&v_full[v_slot], v_phase, quit) && bar_wait(&sh.p_full[0], i & 1, quit);
                     if (!ok) break;
                     fence_after();
-                    second_product(m, i & 1, v_slot, i == 0 || (TERMS == 2 && i % T::flush == 0));
-                    umma_commit(&pv_done[m]);
+                    second_product(0, i & 1, v_slot, fresh);
+                    umma_commit(&pv_done[0]);
+                    next_v();
                 }
-                umma_commit(&v_empty[v_slot]);
-                if (++v_slot == NV) v_slot = 0, v_phase ^= 1;
             }
         }
         // nothing of this CTA's is in flight after this
