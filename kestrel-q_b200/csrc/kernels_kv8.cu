@@ -191,6 +191,38 @@ __device__ __forceinline__ uint32_t encode(float q) {
     }
 }
 
+// Four new values x * (1 / s) -> four stored bytes, if each is what the
+// correctly rounded quotient x / s would give: x * RN(1 / s) is within 3 units
+// of its last place, so only products that near to a rounding border of the
+// format can differ.  `near` is set if one is (the caller divides then).
+// int8: adding 1.5 * 2^23 + 128 rounds to an integer, ties to even, and leaves
+// its low byte with 128 added.  (Dividing every value: 80 us for 48 ragged F32
+// prompts, 40k tokens; this: 58.)
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode4(float4 x, float inv, bool &near) {
+    const float q[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    if constexpr (E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // three mantissa bits: the border is at the middle of the other 20 (subnormals: elsewhere)
+            const uint32_t low = (__float_as_uint(q[i]) + 8u - 0x80000u) & 0xfffffu;
+            near |= low < 16u || fabsf(q[i]) < 0.015625f;
+        }
+        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+        return a | b << 16;
+    } else {
+        uint32_t bits[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float r = __fadd_rn(q[i], 12583040.0f);
+            near |= fabsf(__fsub_rn(q[i], __fsub_rn(r, 12583040.0f))) > 0.4999f;
+            bits[i] = __float_as_uint(r);
+        }
+        return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+    }
+}
+
 template <bool E4M3>
 __device__ __forceinline__ float decode(uint32_t byte) {
     if constexpr (E4M3) {
@@ -280,7 +312,16 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
     auto recode = [&](uint32_t byte) {
         return encode<E4M3>(__fmul_rn(decode<E4M3>(byte), ratio));
     };
-    auto fresh = [&](float x) { return encode<E4M3>(scale > 0.0f ? __fdiv_rn(x, scale) : 0.0f); };
+    auto exact = [&](float x) { return encode<E4M3>(scale > 0.0f ? __fdiv_rn(x, scale) : 0.0f); };
+    // the reciprocal's path wants normal numbers
+    const bool plain = scale < 1.0e-30f || scale > 1.0e30f;
+    const float inv = plain ? 0.0f : __frcp_rn(scale);
+    auto fresh4 = [&](float4 x) {
+        bool near = plain;
+        uint32_t w = encode4<E4M3>(x, inv, near);
+        if (near) w = exact(x.x) | exact(x.y) << 8 | exact(x.z) << 16 | exact(x.w) << 24;
+        return w;
+    };
     for (uint32_t u = g0 * D + tid; u < g1 * D; u += kAppendThreads) {   // D units of 16 bytes in a group
         const uint32_t group = u / D, w = u % D;
         uint4 *unit = reinterpret_cast<uint4 *>(codes + (uint64_t)group * 32 * D + w * 16);
@@ -291,7 +332,7 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float4 x = load4<BF16>(rows, base + (uint64_t)(row - at) * stride + f + 4 * i);
-                    word[i] = fresh(x.x) | fresh(x.y) << 8 | fresh(x.z) << 16 | fresh(x.w) << 24;
+                    word[i] = fresh4(x);
                 }
             } else if (at == 0) {
 #pragma unroll
@@ -323,10 +364,9 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
                 const uint32_t row = t0 + (k >> 1) * 8 + (k & 1), keep = ~(0xffu << (8 * k));
                 if (row >= at && row < end) {
                     const float4 x = load4<BF16>(rows, base + (uint64_t)(row - at) * stride + f);
-                    word[0] = (word[0] & keep) | fresh(x.x) << (8 * k);
-                    word[1] = (word[1] & keep) | fresh(x.y) << (8 * k);
-                    word[2] = (word[2] & keep) | fresh(x.z) << (8 * k);
-                    word[3] = (word[3] & keep) | fresh(x.w) << (8 * k);
+                    const uint32_t four = fresh4(x);   // one byte of each word
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) word[i] = (word[i] & keep) | (four >> (8 * i) & 0xffu) << (8 * k);
                     changed = true;
                 } else if (row < at && grown) {
 #pragma unroll

@@ -714,6 +714,11 @@ namespace {
 
 constexpr uint32_t kSms = 148;
 constexpr uint32_t kShortRows = 64;        // requests up to this many rows go to the row kernel
+// Steps of at most this many units go to the row kernel whole: a prompt tile
+// takes 19 us at least, the row kernel 8 us and about 1.7 ns a unit (7 odd
+// requests, 37 tokens over 333, 10 heads of 64: 27 us in both kernels, 12 in
+// the row kernel alone).
+constexpr uint64_t kFewUnits = 8192;
 constexpr uint32_t kManyPartials = 8;      // shares per tile from which a tile is joined by many CTAs
 constexpr uint32_t kMinPromptGroups = 64;  // a split of a prompt: 1024 tokens or more
 
@@ -779,11 +784,13 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
     const uint64_t groups = std::max<uint64_t>(1, ceil_div(deepest, kG));
     // the longest request, if every request brings a token
     const uint64_t longest = (s.tokens > s.requests ? s.tokens - s.requests : 0) + 1, rows = longest * G;
-    const bool prompts = rows > kShortRows;
+    // 16-row groups that the row kernel would walk if it took everything
+    const uint64_t units = ceil_div((uint64_t)s.tokens * G, 16) * c.heads * groups;
+    const bool prompts = rows > kShortRows && units > kFewUnits;
     h.row_limit = prompts ? kShortRows : UINT32_MAX;
     h.row_tile = rows <= 8 ? 8 : 16;
     // one wave of the row kernel, or shares of at least kMinShare groups
-    const uint64_t tiles = ceil_div(std::min<uint64_t>(rows, kShortRows), h.row_tile);
+    const uint64_t tiles = ceil_div(prompts ? std::min<uint64_t>(rows, kShortRows) : rows, h.row_tile);
     const uint64_t items = s.requests * tiles * c.heads;
     const uint32_t wide = h.row_tile / 8 * c.dim;
     const uint64_t wave = kSms * (wide == 512 ? 2 : c.dim == 256 || wide == 256 ? 3 : 4);

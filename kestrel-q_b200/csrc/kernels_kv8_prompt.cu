@@ -234,7 +234,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
     const uint32_t steps = g1 > g0 ? (g1 - g0 + T::groups - 1) / T::groups : 0u;
     const uint32_t tiles = min((uint32_t)MT, (row_end - row0 + 127) / 128);   // tiles that hold rows
     const int32_t *table = s.table + (uint64_t)b * s.table_stride;
-    const uint32_t per_page = c.page_tokens / kG;
+    const uint32_t page_shift = __ffs(c.page_tokens / kG) - 1;   // groups of a page, a power of two
 
     constexpr uint32_t kMmaWarp = T::softmax_warps + T::widen_warps;
     if (warp == kMmaWarp) {
@@ -364,7 +364,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             // lane l holds the scales of the step's group l; page ids are read two steps ahead, scales one
             auto page_of = [&](uint32_t j) {
                 const uint32_t g = g0 + j * T::groups + lane;
-                return lane < T::groups && j < steps && g < g1 ? table[g / per_page] : -1;
+                return lane < T::groups && j < steps && g < g1 ? table[g >> page_shift] : -1;
             };
             auto scales_of = [&](int32_t id) {   // out of range: the widening warps raise the error
                 return id >= 0 && (uint32_t)id < c.pages
@@ -565,14 +565,14 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         // lane l: where group l's codes are (UINT64_MAX: behind the last); page ids are read two steps ahead
         auto page_of = [&](uint32_t j) {
             const uint32_t g = g0 + j * T::groups + lane;
-            return lane < T::groups && j < steps && g < g1 ? table[g / per_page] : INT32_MIN;
+            return lane < T::groups && j < steps && g < g1 ? table[g >> page_shift] : INT32_MIN;
         };
         auto place_of = [&](uint32_t j, int32_t id) {
             if (id == INT32_MIN) return UINT64_MAX;
             const uint32_t g = g0 + j * T::groups + lane;
             const bool in = id >= 0 && (uint32_t)id < c.pages;
             if (!in) raise(err, kErrStep);
-            return (uint64_t)(((uint64_t)(in ? id : 0) * c.heads + head) * page_bytes + (uint64_t)(g % per_page) * 32 * D);
+            return (uint64_t)(((uint64_t)(in ? id : 0) * c.heads + head) * page_bytes + (uint64_t)(g & ((1u << page_shift) - 1)) * 32 * D);
         };
         uint64_t place = place_of(0, page_of(0));
         int32_t id = page_of(1);
@@ -669,7 +669,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             for (int term = TERMS - 1; term >= 0; --term) {
                 uint64_t qa = q_desc + (m * TERMS + term) * (128 * D / 8);
                 uint64_t kb = k_desc + slot * (T::slot / 16);
-#pragma unroll 1
+#pragma unroll 2
                 for (int f = 0; f < D / 64; ++f, qa += 1024, kb += T::tokens * 8) {
                     umma_ss<T::tokens>(d, qa, kb, more);
                     umma_ss<T::tokens>(d, qa + 2, kb + 2, 1);
