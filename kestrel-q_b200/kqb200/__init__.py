@@ -624,6 +624,7 @@ class Kv8Cache:
                  codes=None, scales=None, device="cuda"):
         import torch
         self._dtypes = {torch.float32: 0, torch.bfloat16: 1}
+        self._int32, self._float32 = torch.int32, torch.float32
         self.kv_heads, self.head_dim, self.page_tokens, self.pages = kv_heads, head_dim, page_tokens, pages
         self.args = abi.Kv8CacheArgs(kv_heads, head_dim, page_tokens, pages, self.FORMATS[format])
         nbytes = lib().kq_b200_kv8_codes_bytes(C.byref(self.args))
@@ -643,21 +644,20 @@ class Kv8Cache:
     def _rows(self, name: str, a, tokens: int, heads: int | None):
         """(dtype, address, token stride) of rows [tokens][heads][head_dim]
         (the stride of a dimension of one element says nothing)."""
-        if a.dim() != 3 or a.shape[0] < tokens or a.shape[2] != self.head_dim or a.stride(2) != 1 \
-                or (a.shape[1] > 1 and a.stride(1) != self.head_dim) or (heads is not None and a.shape[1] != heads):
-            raise ValueError(f"{name}: rows [tokens][heads][{self.head_dim}] with consecutive heads are required")
-        if a.dtype not in self._dtypes:
+        shape, stride, d = a.shape, a.stride(), self.head_dim
+        if len(shape) != 3 or shape[0] < tokens or shape[2] != d or stride[2] != 1 or (shape[1] > 1 and stride[1] != d) \
+                or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name}: rows [tokens][heads][{d}] with consecutive heads are required")
+        dtype = self._dtypes.get(a.dtype)
+        if dtype is None:
             raise ValueError(f"{name}: float32 or bfloat16 is required")
-        return self._dtypes[a.dtype], a.data_ptr(), a.stride(0) if tokens > 1 else a.shape[1] * self.head_dim
+        return dtype, a.data_ptr(), stride[0] if tokens > 1 else shape[1] * d
 
     def plan(self, step: Kv8Step, context_lengths, new_lengths, free_pages, free_head, free_head_out) -> None:
         n = step.args.request_count
-        for name, a, least in (("context_lengths", context_lengths, n), ("new_lengths", new_lengths, n),
-                               ("free_pages", free_pages, 0), ("free_head", free_head, 1),
-                               ("free_head_out", free_head_out, 1)):
-            _tensor(name, a, "int32")
-            if a.numel() < least or not a.is_contiguous():
-                raise ValueError(f"{name}: {least} consecutive values are required")
+        for a, least in ((context_lengths, n), (new_lengths, n), (free_pages, 0), (free_head, 1), (free_head_out, 1)):
+            if a.dtype != self._int32 or a.numel() < least or not a.is_contiguous():
+                raise ValueError("a plan takes consecutive int32 lengths, free pages and heads")
         d = abi.Diagnostic()
         abi.check(lib().kq_b200_kv8_plan(self.args, step.args, context_lengths.data_ptr(), new_lengths.data_ptr(),
                                          free_pages.data_ptr(), free_pages.numel(), free_head.data_ptr(),
@@ -674,10 +674,8 @@ class Kv8Cache:
 
     def read_pages(self, pages, values) -> None:
         """values (float32 [pages][heads][key, value][page_tokens][head_dim]) of the page ids `pages` (int32)."""
-        _tensor("pages", pages, "int32")
-        _tensor("values", values, "float32")
-        if not (pages.is_contiguous() and values.is_contiguous()):
-            raise ValueError("pages and values must be contiguous")
+        if pages.dtype != self._int32 or values.dtype != self._float32 or not (pages.is_contiguous() and values.is_contiguous()):
+            raise ValueError("contiguous int32 pages and float32 values are required")
         d = abi.Diagnostic()
         abi.check(lib().kq_b200_kv8_read(self.args, pages.data_ptr(), pages.numel(), values.data_ptr(), values.numel(),
                                          C.byref(d)), d)
@@ -699,9 +697,8 @@ class Kv8Cache:
         if qt != ot:
             raise ValueError("query and output must have the same type")
         if lse is not None:
-            _tensor("lse", lse, "float32")
-            if lse.numel() < n * query.shape[1] or not lse.is_contiguous():
-                raise ValueError("lse: one value per token and query head is required")
+            if lse.dtype != self._float32 or lse.numel() < n * query.shape[1] or not lse.is_contiguous():
+                raise ValueError("lse: one float32 per token and query head is required")
         if workspace is not None and not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         d = abi.Diagnostic()
@@ -712,7 +709,8 @@ class Kv8Cache:
 
 
 def _tensor(name: str, a, dtype: str):
-    if str(a.dtype) != "torch." + dtype:
+    import torch
+    if a.dtype != getattr(torch, dtype):
         raise ValueError(f"{name}: {dtype} is required")
     return a
 

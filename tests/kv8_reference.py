@@ -113,18 +113,20 @@ def attend(cache, table, context, new, q, scale):
     size, top = np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     row = 0
     for b, (c, n) in enumerate(zip(context, new)):
-        kv = cache.rows(table[b], max(0, c + n))
-        for i in range(n):
-            seen = c + i + 1
-            for h in range(q.shape[1] if seen > 0 else 0):
-                k, v = kv[0, h // G, :seen], kv[1, h // G, :seen]
-                x = q[row + i, h].astype(np.float64)
-                l = k @ x * scale
-                m = l.max()
+        if n and c + n > 0:
+            kv = cache.rows(table[b], c + n)
+            hidden = np.arange(c + n) > c + np.arange(n)[:, None]
+            some = ~hidden.all(1)   # rows that see something
+            for h in range(q.shape[1]):
+                k, v = kv[:, h // G]
+                x = q[row:row + n, h].astype(np.float64)
+                l = np.where(hidden, -np.inf, x @ k.T * scale)[some]
+                m = l.max(1, keepdims=True)
                 w = np.exp(l - m)
-                out[row + i, h] = w @ v / w.sum()
-                lse[row + i, h] = m + np.log(w.sum())
-                size[row + i, h] = (np.abs(k) @ np.abs(x)).max() * abs(scale)
-                top[row + i, h] = np.abs(v).max()
+                at = np.arange(row, row + n)[some]
+                out[at, h] = w @ v / w.sum(1, keepdims=True)
+                lse[at, h] = (m + np.log(w.sum(1, keepdims=True)))[:, 0]
+                size[at, h] = np.where(hidden, 0, np.abs(x) @ np.abs(k).T)[some].max(1) * abs(scale)
+                top[at, h] = np.where(hidden[some], 0, np.abs(v).max(1)).max(1)
         row += n
     return out, lse, size, top

@@ -116,15 +116,20 @@ class Server:
         scale = 1 / math.sqrt(self.dim) if scale is None else scale
         host = self.rng.standard_normal((tokens, query_heads, self.dim)).astype(np.float32) if q is None else q
         host[T:] = np.nan
-        qd = dev(host, dtype)
-        out = torch.full_like(qd, 7.0)
+        # queries and outputs inside wider rows, of which nothing else may change
+        qw = torch.full((tokens, query_heads + 2, self.dim), math.nan, dtype=getattr(torch, dtype), device="cuda")
+        qd = qw[:, 1:-1]
+        qd.copy_(torch.as_tensor(host))
+        wide = torch.full_like(qw, 7.0)
+        out = wide[:, 1:-1]
         lse = torch.full((tokens, query_heads), 7.0, device="cuda")
         ws = torch.empty(self.cache.attend_workspace_bytes(step, query_heads, hint), dtype=torch.uint8, device="cuda")
         ws.fill_(255)   # NaNs: partials must be written before they are read
         torch.cuda.synchronize()
         self.cache.attend(step, qd, out, lse, scale=scale, max_kv_length=hint, workspace=ws)
         self.kq.synchronize()
-        assert torch.all(out[T:] == 7) and torch.all(lse[T:] == 7)
+        assert torch.all(wide[T:] == 7) and torch.all(lse[T:] == 7)
+        assert torch.all(wide[:, 0] == 7) and torch.all(wide[:, -1] == 7)
         got, got_lse = out[:T].float().cpu().numpy(), lse[:T].cpu().numpy()
         if check:
             before = [c - n for c, n in zip(self.context, new)]
@@ -351,6 +356,105 @@ def test_attention_over_long_contexts(kq, dtype, hint):
     new = [40, 30, 0]   # 160 and 120 rows: the prompt kernel, split
     step = s.step(new)
     s.attend(step, new, 4, hint=hint)
+
+
+class Launches:
+    """Launches of a kernel family while it is watched."""
+
+    def __init__(self, kq, family):
+        self.kq, self.family = kq, family
+
+    def __enter__(self):
+        self.kq.lib().kq_b200_profile_kernel(self.family.encode())
+        return self
+
+    def __exit__(self, *_):
+        n, ms = C.c_uint64(), C.c_double()
+        self.kq.lib().kq_b200_profile_read(C.byref(n), C.byref(ms))
+        self.kq.lib().kq_b200_profile_kernel(None)
+        self.count = n.value
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,queries,dim,page", [(2, 16, 256, 64), (2, 6, 128, 16), (1, 24, 64, 32), (3, 3, 128, 128)])
+def test_prompts(kq, fmt, dtype, heads, queries, dim, page):
+    """Long prompts and chunks beside decode tokens in one step: tiles that
+    end in mid-tile, both attention kernels, pages smaller and larger than a
+    step of the prompt kernel."""
+    s = Server(kq, heads, dim, page, fmt, 5, -(-4000 // page), pages=5 * -(-700 // page), seed=queries, dtype=dtype)
+    for new, padding in (([300, 1, 0, 37, 165], 0), ([90, 1, 130, 2, 1], 21)):
+        step = s.step(new, padding)
+        with Launches(kq, "kv8_prompt") as seen:
+            s.attend(step, new, queries)
+        assert seen.count == 1
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim,queries", [(64, 3), (128, 8), (256, 5)])
+def test_prompts_over_long_contexts(kq, dtype, dim, queries):
+    """Key axes cut into splits, F32 sums moved out on the way, and the same
+    over one split (many tiles)."""
+    s = Server(kq, 1, dim, 64, "int8", 3, 110, seed=dim, dtype=dtype)
+    s.step([5000, 1300, 0])
+    for new in ([90, 70, 0], [1, 200, 150]):
+        step = s.step(new)
+        with Launches(kq, "kv8_prompt") as seen:
+            s.attend(step, new, queries)
+        assert seen.count == 1
+    s = Server(kq, 8, dim, 64, "e4m3", 1, 110, seed=dim, dtype=dtype)
+    s.step([1100])
+    new = [700]
+    step = s.step(new)
+    with Launches(kq, "kv8_prompt") as seen:
+        s.attend(step, new, 8 * 5)
+    assert seen.count == 1
+
+
+def test_prompts_of_bad_contents(kq):
+    """What the prompt kernel refuses, and that it works after it."""
+    import torch
+    for what in ("query", "page", "length"):
+        s = Server(kq, 1, 128, 16, "e4m3", 2, 200, pages=60)
+        s.step([50, 20])
+        new = [300, 1]
+        step = s.step(new)
+        q = torch.randn(301, 8, 128, device="cuda")
+        out = torch.empty_like(q)
+        ws = torch.empty(s.cache.attend_workspace_bytes(step, 8), dtype=torch.uint8, device="cuda")
+        table, lengths = s.table_dev.clone(), step.kv_lengths.clone()
+        if what == "query":
+            q[299, 7, 127] = math.nan
+        elif what == "page":
+            s.table_dev[0, 17] = -1
+        else:
+            step.kv_lengths[0] = 200 * 16 + 1
+        torch.cuda.synchronize()
+        with Launches(kq, "kv8_prompt") as seen:
+            s.cache.attend(step, q, out, scale=0.1, workspace=ws)
+            with pytest.raises(kq.KQError) as e:
+                kq.synchronize()
+        assert seen.count == 1
+        assert e.value.status == (kq.abi.NUMERIC_DOMAIN if what == "query" else kq.abi.SPAN_OUT_OF_RANGE)
+        s.table_dev.copy_(table)
+        step.kv_lengths.copy_(lengths)
+        s.attend(step, new, 8)
+
+
+def test_two_threads(kq):
+    """Two threads with a cache each: calls are ordered by the library."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def serve(seed):
+        s = Server(kq, 2, 64, 16, "int8", 2, 30, seed=seed)
+        s.step([100, 37])
+        for _ in range(4):
+            step = s.step([1, 1])
+            s.attend(step, [1, 1], 4)
+        return True
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(serve, [1, 2]))
 
 
 @pytest.mark.parametrize("queries", [8, 64])
