@@ -616,7 +616,8 @@ typedef struct kq_b200_kv8_cache {
  *          feature 64 j + 16 t + e, token 8 h + g
  *   value  [j: d/32][g: 8][t: 4][i: 4][h: 2][e: 2]
  *          feature 32 j + 4 g + i, token 8 h + 2 t + e
- * An int8 code is stored with 128 added.  0 if the geometry is not
+ * An int8 code is stored with 128 added.  A new cache holds code 0 (bytes 128
+ * or 0) and scale 0; e4m3 codes are never NaN.  0 if the geometry is not
  * supported. */
 uint64_t kq_b200_kv8_codes_bytes(const kq_b200_kv8_cache *cache);
 uint64_t kq_b200_kv8_scales_count(const kq_b200_kv8_cache *cache);

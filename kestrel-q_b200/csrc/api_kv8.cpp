@@ -102,6 +102,8 @@ kq_status check_step(const kq_b200_kv8_step *s, Kv8Step *out, kq_diagnostic *d) 
         return fail(d, KQ_STATUS_LIMIT_EXCEEDED, "a step has at most 16384 requests and 2^31 - 1 tokens");
     if (s->table_stride < s->table_columns)
         return fail(d, KQ_STATUS_DIMENSION_MISMATCH, "block table stride is below its columns");
+    if (s->table_stride > (uint64_t)INT64_MAX / 4 / s->request_count)
+        return fail(d, KQ_STATUS_ARITHMETIC_OVERFLOW, "block table overflows the address space");
     out->requests = s->request_count;
     out->tokens = s->token_capacity;
     out->columns = s->table_columns;

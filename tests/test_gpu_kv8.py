@@ -146,7 +146,7 @@ class Server:
 # ------------------------------------------------------------------- plan
 
 @pytest.mark.parametrize("requests,page,most", [(1, 16, 1), (1, 64, 5000), (7, 16, 40), (64, 64, 1), (300, 32, 90),
-                                                (1025, 128, 9), (2000, 16, 3)])
+                                                (1025, 128, 9), (2000, 16, 3), (16384, 32, 2)])
 def test_plan(kq, requests, page, most):
     import torch
     rng = np.random.default_rng(requests)

@@ -87,7 +87,8 @@ def test_refused_cache_arrays(kq, over, want):
                                        (dict(table_columns=0), "INVALID_ARGUMENT"),
                                        (dict(request_count=16385), "LIMIT_EXCEEDED"),
                                        (dict(token_capacity=1 << 31), "LIMIT_EXCEEDED"),
-                                       (dict(table_stride=3), "DIMENSION_MISMATCH")])
+                                       (dict(table_stride=3), "DIMENSION_MISMATCH"),
+                                       (dict(table_stride=1 << 62), "ARITHMETIC_OVERFLOW")])
 def test_refused_steps(kq, over, want):
     s = _step(kq, **over)
     assert {plan(kq, step=s), append(kq, step=s), attend(kq, step=s)} == {getattr(kq.abi, want)}
