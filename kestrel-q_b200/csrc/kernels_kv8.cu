@@ -1,23 +1,25 @@
 // Paged 8-bit key/value cache: the plan of a ragged step, the append of new
 // rows and the read-out of pages.  (The attention: kernels_kv8_attend.cu.)
-#include "kernels_kv8.hpp"
+#include "kernels_kv8.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 namespace kqb {
 
 namespace {
 
-__device__ __forceinline__ bool kv8_err_raised(const ErrorWord &e) {
-    return *reinterpret_cast<volatile unsigned long long *>(e.word) != 0ull;
-}
-
-__device__ __forceinline__ void kv8_raise(const ErrorWord &e, uint32_t code) {
-    atomicCAS(e.word, 0ull, ((unsigned long long)code << 32) | e.call_id);
+// go(integral constant) for the head dimension: the layout's divisions are shifts then
+template <class Go>
+void by_dimension(uint32_t dim, Go go) {
+    if (dim == 256)
+        go(std::integral_constant<int, 256>());
+    else if (dim == 128)
+        go(std::integral_constant<int, 128>());
+    else
+        go(std::integral_constant<int, 64>());
 }
 
 // ------------------------------------------------------------------- plan
@@ -48,7 +50,7 @@ kv8_plan_kernel(Kv8Cache c, Kv8Step s, Kv8Plan p, ErrorWord err) {
     const uint32_t B = s.requests, P = c.page_tokens, tid = threadIdx.x;
     int32_t *off = plan_smem, *taken = off + B + 1, *runs = taken + B + 1;
     pdl_wait();
-    if (__syncthreads_or(tid == 0 && kv8_err_raised(err))) return;
+    if (__syncthreads_or(tid == 0 && err_raised(err))) return;
 
     // consecutive requests per thread; sums in 64 bits until they are checked
     const uint32_t per = (B + kPlanThreads - 1) / kPlanThreads;
@@ -97,7 +99,7 @@ kv8_plan_kernel(Kv8Cache c, Kv8Step s, Kv8Plan p, ErrorWord err) {
     const long long head = p.free_head[0];
     bad |= total[0] > s.tokens || total[2] > s.runs || head < 0 || head + total[1] > p.free_count;
     if (bad) {   // the same for every thread of every CTA: nothing is written
-        if (tid == 0) kv8_raise(err, kErrStep);
+        if (tid == 0) raise(err, kErrStep);
         return;
     }
     for (uint32_t b = b0; b < b1; ++b) {
@@ -144,7 +146,7 @@ kv8_plan_kernel(Kv8Cache c, Kv8Step s, Kv8Plan p, ErrorWord err) {
         const bool fresh = column >= first;
         const int32_t page = fresh ? p.free_pages[head + taken[lo] + (column - first)] : *entry;
         const bool ok = page >= 0 && (uint32_t)page < c.pages;
-        if (!ok) kv8_raise(err, kErrStep);
+        if (!ok) raise(err, kErrStep);
         if (ok && fresh && pos % P == 0) *entry = page;
         s.slots[t] = ok ? (int64_t)page * P + pos % P : -1;
         s.positions[t] = (int32_t)pos;
@@ -172,17 +174,6 @@ namespace {
 constexpr int kAppendThreads = 256;
 constexpr uint32_t kAhead = 4;
 
-template <bool BF16>
-__device__ __forceinline__ float4 load4(const void *base, uint64_t at) {
-    if constexpr (BF16) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(base) + at);
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                           __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-    } else {
-        return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-    }
-}
-
 // The stored byte of an F32 quotient: nearest, ties to even, clamped to the
 // format's range (a scale that is itself subnormal can be rounded down).
 template <bool E4M3>
@@ -194,36 +185,35 @@ __device__ __forceinline__ uint32_t encode(float q) {
     }
 }
 
-// Four new values x * (1 / s) -> four stored bytes, if each is what the
-// correctly rounded quotient x / s would give: x * RN(1 / s) is within 3 units
-// of its last place, so only products that near to a rounding border of the
-// format can differ.  `near` is set if one is (the caller divides then).
-// int8: adding 1.5 * 2^23 + 128 rounds to an integer, ties to even, and leaves
-// its low byte with 128 added.  (Dividing every value: 80 us for 48 ragged F32
-// prompts, 50k tokens; this: 65.)
+// Four new values -> four stored bytes, from two products each: with inv the
+// rounded 1 / s, low = inv (1 - 2^-22) and high = inv (1 + 2^-22) hold the
+// correctly rounded quotient x / s between them, and rounding to the format
+// keeps that order.  So where both give one code it is the quotient's; `near`
+// is set where they differ (the caller divides then).
+// int8: adding 1.5 * 2^23 + 128 rounds the product to an integer, ties to even,
+// and leaves its low byte with 128 added.  (Dividing every value: 80 us for 48
+// ragged F32 prompts, 50k tokens; this: 60.)
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode4(float4 x, float inv, bool &near) {
-    const float q[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-    if constexpr (E4M3) {
+__device__ __forceinline__ uint32_t encode4(float4 x, float low, float high, bool &near) {
+    const uint64_t xy = pack2(x.x, x.y), zw = pack2(x.z, x.w);
+    uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // three mantissa bits: the border is at the middle of the other 20 (subnormals: elsewhere)
-            const uint32_t low = (__float_as_uint(q[i]) + 8u - 0x80000u) & 0xfffffu;
-            near |= low < 16u || fabsf(q[i]) < 0.015625f;
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t by = i == 0 ? pack2(low, low) : pack2(high, high);
+        float a, b, c, d;
+        if constexpr (E4M3) {
+            unpack2(mul2(xy, by), a, b), unpack2(mul2(zw, by), c, d);
+            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+        } else {
+            const uint64_t to = pack2(12583040.0f, 12583040.0f);
+            unpack2(fma2(xy, by, to), a, b), unpack2(fma2(zw, by, to), c, d);
+            w[i] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                               __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
         }
-        const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-        return a | b << 16;
-    } else {
-        uint32_t bits[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float r = __fadd_rn(q[i], 12583040.0f);
-            near |= fabsf(__fsub_rn(q[i], __fsub_rn(r, 12583040.0f))) > 0.4999f;
-            bits[i] = __float_as_uint(r);
-        }
-        return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
     }
+    near |= w[0] != w[1];
+    return w[0];
 }
 
 template <bool E4M3>
@@ -255,46 +245,49 @@ template <bool E4M3> constexpr uint32_t kZeroByte = E4M3 ? 0u : 128u;
 // Bound: HBM and the instructions of the rounding for prompts, latency for
 // single tokens (one group of 16 tokens is touched unless the scale grows).
 // Measured under ncu, caches cold: 48 ragged F32 prompts, 50k tokens of 2 x 256
-// features, 65 us (257 MB: 3.9 TB/s); an 8k bf16 prompt of 8 x 128, e4m3, 30 us
-// (50 MB); 64 decode tokens 6.3 us.
-template <bool E4M3, bool BF16>
+// features, 60 us (257 MB: 4.3 TB/s); an 8k bf16 prompt of 8 x 128, e4m3, 25 us
+// (50 MB, three quarters of the issue slots); 64 decode tokens 5.9 us.  Indexes of
+// compile-time head dimensions and page shifts: 65, 30 and 6.3 us with divisions.
+// A thread's places of a group kept across groups took registers (48 for 36) and
+// lost (63 and 28 us under the same profile that gives this 62 and 27).
+template <int D, bool E4M3, bool BF16>
 __global__ void __launch_bounds__(kAppendThreads)
 kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, const void *values, uint64_t v_stride,
                   ErrorWord err) {
-    __shared__ uint32_t warp_max[kAppendThreads / 32];
-    __shared__ uint32_t run_rows;
-    const uint32_t tid = threadIdx.x, P = c.page_tokens, D = c.dim;
+    __shared__ uint32_t warp_max[kAppendThreads / 32], warp_rows[kAppendThreads / 32];
+    constexpr uint32_t quads = D / 4;
+    const uint32_t tid = threadIdx.x, P = c.page_tokens;
     const uint32_t head = blockIdx.y >> 1, side = blockIdx.y & 1u;
     pdl_wait();
+    // the slots and the first rows are on their way while the run is looked at
     const int32_t first = s.page_runs[blockIdx.x];
-    if (__syncthreads_or(first < 0 || (tid == 0 && kv8_err_raised(err)))) return;
-    if ((uint32_t)first >= s.tokens) {
-        if (tid == 0) kv8_raise(err, kErrStep);
-        return;
-    }
-    const int64_t slot = s.slots[first];
+    const uint32_t room = (uint32_t)first < s.tokens ? min(P, s.tokens - (uint32_t)first) : 0u;
+    const int64_t slot = room > 0 ? s.slots[first] : -1, mine = tid < room ? s.slots[first + tid] : -1;
     const void *rows = side ? values : keys;
     const uint64_t stride = side ? v_stride : k_stride, base = (uint64_t)first * stride + (uint64_t)head * D;
-    const uint32_t quads = D / 4;
-    // the first rows are on their way while the slots are looked at
     float4 ahead[kAhead];
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; ++i) {
         const uint32_t row = (tid + i * kAppendThreads) / quads, f = (tid + i * kAppendThreads) % quads * 4;
         ahead[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (row < min(P, s.tokens - (uint32_t)first)) ahead[i] = load4<BF16>(rows, base + row * stride + f);
+        if (row < room) ahead[i] = load4<BF16>(rows, base + row * stride + f);
     }
-    if (slot < 0 || slot >= (int64_t)c.pages * P) {
-        if (tid == 0) kv8_raise(err, kErrStep);
+    if (__syncthreads_or(first < 0 || (tid == 0 && err_raised(err)))) return;
+    if (slot < 0 || slot >= (int64_t)c.pages * P) {   // no room: first is behind the rows
+        if (tid == 0) raise(err, kErrStep);
         return;
     }
-    const uint64_t page = (uint64_t)slot / P;
-    const uint32_t at = (uint32_t)((uint64_t)slot % P), most = min(P - at, s.tokens - (uint32_t)first);
-    if (tid == 0) run_rows = most;
+    const uint32_t page_shift = __ffs(P) - 1;   // a power of two
+    const uint64_t page = (uint64_t)slot >> page_shift;
+    const uint32_t at = (uint32_t)slot & (P - 1), most = min(P - at, room);
+    // the run ends before the first row whose slot does not follow
+    const uint32_t other = __ballot_sync(~0u, tid >= most || mine != slot + (int64_t)tid);
+    if ((tid & 31) == 0) warp_rows[tid >> 5] = other != 0 ? tid + __ffs(other) - 1 : P;
     __syncthreads();
-    if (tid < most && s.slots[first + tid] != slot + (int64_t)tid) atomicMin(&run_rows, tid);
-    __syncthreads();
-    const uint32_t n = run_rows, end = at + n;
+    uint32_t n = P;
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) n = min(n, warp_rows[w]);
+    const uint32_t end = at + n;
 
     // |x| as integers order like the floats, infinities and NaNs above all
     uint32_t top = 0;
@@ -316,7 +309,7 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, warp_max[w]);
     if (top >= 0x7f800000u) {   // a non-finite value: this page keeps what it holds
-        if (tid == 0) kv8_raise(err, kErrNonFinite);
+        if (tid == 0) raise(err, kErrNonFinite);
         return;
     }
     const float scale = fmaxf(old, __fdiv_rn(__uint_as_float(top), kLargest<E4M3>));
@@ -335,9 +328,10 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
     // the reciprocal's path wants normal numbers
     const bool plain = scale < 1.0e-30f || scale > 1.0e30f;
     const float inv = plain ? 0.0f : __frcp_rn(scale);
+    const float low = inv * (1.0f - 0x1p-22f), high = inv * (1.0f + 0x1p-22f);
     auto fresh4 = [&](float4 x) {
         bool near = plain;
-        uint32_t w = encode4<E4M3>(x, inv, near);
+        uint32_t w = encode4<E4M3>(x, low, high, near);
         if (near) w = exact(x.x) | exact(x.y) << 8 | exact(x.z) << 16 | exact(x.w) << 24;
         return w;
     };
@@ -385,7 +379,8 @@ kv8_append_kernel(Kv8Cache c, Kv8Step s, const void *keys, uint64_t k_stride, co
                     const float4 x = load4<BF16>(rows, base + (uint64_t)(row - at) * stride + f);
                     const uint32_t four = fresh4(x);   // one byte of each word
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) word[i] = (word[i] & keep) | (four >> (8 * i) & 0xffu) << (8 * k);
+                    for (int i = 0; i < 4; ++i)   // byte k of the word becomes byte i of the four
+                        word[i] = __byte_perm(word[i], four, (0x3210u & ~(0xfu << (4 * k))) | (4u + i) << (4 * k));
                     changed = true;
                 } else if (row < at && grown) {
 #pragma unroll
@@ -406,10 +401,14 @@ void launch_kv8_append(const Kv8Cache &c, const Kv8Step &s, const void *k, uint6
     KernelTimer timer("kv8_append", stream);
     const dim3 grid(s.runs, 2 * c.heads);
     auto go = [&](auto kernel) { launch_pdl(kernel, grid, kAppendThreads, 0, stream, c, s, k, k_stride, v, v_stride, err); };
-    if (c.e4m3)
-        bf16 ? go(kv8_append_kernel<true, true>) : go(kv8_append_kernel<true, false>);
-    else
-        bf16 ? go(kv8_append_kernel<false, true>) : go(kv8_append_kernel<false, false>);
+    auto typed = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        if (c.e4m3)
+            bf16 ? go(kv8_append_kernel<D, true, true>) : go(kv8_append_kernel<D, true, false>);
+        else
+            bf16 ? go(kv8_append_kernel<D, false, true>) : go(kv8_append_kernel<D, false, false>);
+    };
+    by_dimension(c.dim, typed);
     count_launch();
 }
 
@@ -417,51 +416,70 @@ void launch_kv8_append(const Kv8Cache &c, const Kv8Step &s, const void *k, uint6
 
 namespace {
 constexpr int kReadThreads = 256;
+constexpr uint32_t kReadUnits = 4;   // of 16 values, per thread
 }
 
 // The F32 values code * scale of pages[i], natural order: out
-// [i][head][key, value][token][feature].  One CTA per (page, head, side);
-// a thread turns 4 key bytes into 4 features of a token, or 16 value bytes
-// into 4 features of 4 tokens, so that 128 contiguous bytes or more are
-// written together.  Bound: HBM (4 bytes written per byte read).  Measured under
-// ncu, caches cold: 835 pages of 64 tokens, 2 x 256 features, 49 us for 274 MB
-// (5.6 TB/s).
-template <bool E4M3>
+// [i][head][key, value][token][feature].  One CTA per (page, head, side) and
+// 16 K values; a thread turns 4 key bytes into 4 features of a token, or 16
+// value bytes into 4 features of 4 tokens, so that 128 contiguous bytes or more
+// are written together; all its loads are on their way before the first store.
+// Bound: HBM (4 bytes written per byte read).  Measured under ncu, caches cold:
+// 835 pages of 64 tokens, 2 x 256 features, 47 us for 274 MB (5.8 TB/s); 64 such
+// pages 6.7 us (11.7 with a CTA per page side that loads as it goes).  16, 32 and
+// 64 values a thread: 61, 51 and 50 us for the 835 pages by events.
+template <int D, bool E4M3>
 __global__ void __launch_bounds__(kReadThreads)
 kv8_read_kernel(Kv8Cache c, const int32_t *__restrict__ pages, float *__restrict__ out, ErrorWord err) {
-    const uint32_t P = c.page_tokens, D = c.dim, head = blockIdx.y >> 1, side = blockIdx.y & 1u;
+    const uint32_t P = c.page_tokens, head = blockIdx.y >> 1, side = blockIdx.y & 1u;
     pdl_wait();
-    if (kv8_err_raised(err)) return;
     const int32_t page = pages[blockIdx.x];
+    if (err_raised(err)) return;
     if (page < 0 || (uint32_t)page >= c.pages) {
-        if (threadIdx.x == 0) kv8_raise(err, kErrStep);
+        if (threadIdx.x == 0) raise(err, kErrStep);
         return;
     }
     const uint8_t *codes = c.codes + ((uint64_t)page * c.heads + head) * (2ull * P * D) + side * 16u * D;
     const float scale = c.scales[((uint64_t)page * c.heads + head) * 2 + side];
     float *o = out + (((uint64_t)blockIdx.x * c.heads + head) * 2 + side) * P * D;
     if (side == 0) {
-        for (uint32_t u = threadIdx.x; u < P * D / 4; u += kReadThreads) {
+        uint32_t b[4 * kReadUnits];
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kReadUnits; ++i) {
+            const uint32_t u = (blockIdx.z * 4 * kReadUnits + i) * kReadThreads + threadIdx.x;
             const uint32_t row = u / (D / 4), f = u % (D / 4) * 4, w = row % 16;
-            const uint32_t b = *reinterpret_cast<const uint32_t *>(codes + (uint64_t)(row / 16) * 32 * D + f / 64 * 1024 +
-                                                                   w / 8 * 512 + w % 8 * 64 + f % 64);
-            reinterpret_cast<float4 *>(o)[u] =
-                make_float4(__fmul_rn(decode<E4M3>(b & 0xffu), scale), __fmul_rn(decode<E4M3>(b >> 8 & 0xffu), scale),
-                            __fmul_rn(decode<E4M3>(b >> 16 & 0xffu), scale), __fmul_rn(decode<E4M3>(b >> 24), scale));
+            if (row < P)
+                b[i] = *reinterpret_cast<const uint32_t *>(codes + (uint64_t)(row / 16) * 32 * D + f / 64 * 1024 + w / 8 * 512 +
+                                                           w % 8 * 64 + f % 64);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kReadUnits; ++i) {
+            const uint32_t u = (blockIdx.z * 4 * kReadUnits + i) * kReadThreads + threadIdx.x;
+            if (u < P * D / 4)
+                reinterpret_cast<float4 *>(o)[u] =
+                    make_float4(__fmul_rn(decode<E4M3>(b[i] & 0xffu), scale), __fmul_rn(decode<E4M3>(b[i] >> 8 & 0xffu), scale),
+                                __fmul_rn(decode<E4M3>(b[i] >> 16 & 0xffu), scale), __fmul_rn(decode<E4M3>(b[i] >> 24), scale));
         }
     } else {
-        for (uint32_t u = threadIdx.x; u < P * D / 16; u += kReadThreads) {
-            const uint32_t group = u / D, w = u % D;
-            const uint4 b = *reinterpret_cast<const uint4 *>(codes + (uint64_t)group * 32 * D + w * 16);
-            const uint32_t f = w / 32 * 32 + w % 32 / 4 * 4, t0 = group * 16 + w % 4 * 2;
+        uint4 b[kReadUnits];
+#pragma unroll
+        for (uint32_t i = 0; i < kReadUnits; ++i) {
+            const uint32_t u = (blockIdx.z * kReadUnits + i) * kReadThreads + threadIdx.x;
+            if (u < P * D / 16) b[i] = *reinterpret_cast<const uint4 *>(codes + (uint64_t)(u / D) * 32 * D + u % D * 16);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kReadUnits; ++i) {
+            const uint32_t u = (blockIdx.z * kReadUnits + i) * kReadThreads + threadIdx.x, w = u % D;
+            const uint32_t f = w / 32 * 32 + w % 32 / 4 * 4, t0 = u / D * 16 + w % 4 * 2;
+            if (u >= P * D / 16) break;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t row = t0 + (k >> 1) * 8 + (k & 1);
                 *reinterpret_cast<float4 *>(o + (uint64_t)row * D + f) =
-                    make_float4(__fmul_rn(decode<E4M3>(b.x >> (8 * k) & 0xffu), scale),
-                                __fmul_rn(decode<E4M3>(b.y >> (8 * k) & 0xffu), scale),
-                                __fmul_rn(decode<E4M3>(b.z >> (8 * k) & 0xffu), scale),
-                                __fmul_rn(decode<E4M3>(b.w >> (8 * k) & 0xffu), scale));
+                    make_float4(__fmul_rn(decode<E4M3>(b[i].x >> (8 * k) & 0xffu), scale),
+                                __fmul_rn(decode<E4M3>(b[i].y >> (8 * k) & 0xffu), scale),
+                                __fmul_rn(decode<E4M3>(b[i].z >> (8 * k) & 0xffu), scale),
+                                __fmul_rn(decode<E4M3>(b[i].w >> (8 * k) & 0xffu), scale));
             }
         }
     }
@@ -470,11 +488,15 @@ kv8_read_kernel(Kv8Cache c, const int32_t *__restrict__ pages, float *__restrict
 void launch_kv8_read(const Kv8Cache &c, const int32_t *pages, uint32_t count, float *out, ErrorWord err,
                      cudaStream_t stream) {
     KernelTimer timer("kv8_read", stream);
-    const dim3 grid(count, 2 * c.heads);
-    if (c.e4m3)
-        launch_pdl(kv8_read_kernel<true>, grid, kReadThreads, 0, stream, c, pages, out, err);
-    else
-        launch_pdl(kv8_read_kernel<false>, grid, kReadThreads, 0, stream, c, pages, out, err);
+    const uint32_t each = 16 * kReadUnits * kReadThreads;   // values of a CTA
+    const dim3 grid(count, 2 * c.heads, (c.page_tokens * c.dim + each - 1) / each);
+    by_dimension(c.dim, [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        if (c.e4m3)
+            launch_pdl(kv8_read_kernel<D, true>, grid, kReadThreads, 0, stream, c, pages, out, err);
+        else
+            launch_pdl(kv8_read_kernel<D, false>, grid, kReadThreads, 0, stream, c, pages, out, err);
+    });
     count_launch();
 }
 
