@@ -20,12 +20,12 @@
 // against the output's own 2^-9.  The page scales multiply the accumulators
 // (sK) and the weights (sV), never the codes.
 //
-// Softmax in base 2, one pass: the reference point m of a row is raised only
-// when a logit exceeds it by more than 8, so weights stay below 2^8 and the
+// Softmax in base 2, one pass: a row's reference point m is raised only when
+// a logit exceeds it by more than 8, so weights stay below 2^8 and the
 // accumulators are rarely rescaled; m, the sums l and O are F32.  The weights
-// entering the second product are p * sV / R * 2^6 with R the smallest power
-// of two not below any sV seen (O is rescaled exactly when R grows): at most
-// 2^14, and anything below 2^-24 of that is lost (2^-38 of the largest).
+// entering the second product are p * sV against a reference point of their
+// own (kernels_kv8.cuh): at most 2^14, the row's largest 2^5 or more, so what
+// fp16 cannot hold of a weight is below 2^-30 of the row's largest.
 //
 // Layout.  A page keeps its codes in the order the fragments need (see
 // Kv8Cache), so a warp reads both operands with conflict-free 16-byte shared
@@ -126,14 +126,13 @@ constexpr uint32_t kRowSmem = kRowWarps * kRowStages<D, NT> * 32 * D + NT * TERM
 template <int D, int NT>
 struct Columns {
     float o[NT][D / 16][4];
-    float m[NT][2], l[NT][2], ref;
+    float m[NT][2], mo[NT][2], l[NT][2];
 
     __device__ __forceinline__ void clear() {
-        ref = 0.0f;
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) m[a][r] = -INFINITY, l[a][r] = 0.0f;
+            for (int r = 0; r < 2; ++r) m[a][r] = mo[a][r] = -INFINITY, l[a][r] = 0.0f;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
 #pragma unroll
@@ -184,6 +183,7 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
         }
     }
     float s[NT][4], top[NT][2];
+    const float size = size_of(vs);
     bool lift = false;
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
@@ -202,7 +202,7 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
             top[a][r] = x;
-            lift |= x > st.m[a][r] + kRaise;
+            lift |= x > st.m[a][r] + kRaise || x + size > st.mo[a][r] + kRaise;
         }
     }
     if (__any_sync(~0u, lift)) {   // -inf + 8 is -inf: the first finite logit of a row lifts it
@@ -211,10 +211,15 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
             float by[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float m = fmaxf(st.m[a][r], top[a][r]);
-                by[r] = m == -INFINITY ? 1.0f : exp2_approx(st.m[a][r] - m);
+                const float m = fmaxf(st.m[a][r], ceilf(top[a][r])), mo = fmaxf(st.mo[a][r], ceilf(top[a][r] + size));
+                if (m == -INFINITY) {
+                    by[r] = 1.0f;
+                    continue;
+                }
+                st.l[a][r] *= exp2_approx(st.m[a][r] - m);
+                by[r] = exp2_approx(st.mo[a][r] - mo);
                 st.m[a][r] = m;
-                st.l[a][r] *= by[r];
+                st.mo[a][r] = mo;
             }
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
@@ -222,29 +227,16 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
                 for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by[k & 1];
         }
     }
-    if (vs > st.ref) {
-        // the next power of two, within the normal range
-        const uint32_t e = min((__float_as_uint(vs) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
-        const float ref = __uint_as_float(max(e, 0x00800000u));
-        const float by = st.ref / ref;
-        st.ref = ref;
-#pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) st.o[a][n][k] *= by;
-    }
-    const float w = st.ref > 0.0f ? vs * (kWeightScale / st.ref) : 0.0f;
     uint2 p[NT][TERMS];
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
         float e[4];
+        const float w[2] = {weight_of(st.m[a][0], st.mo[a][0]) * vs, weight_of(st.m[a][1], st.mo[a][1]) * vs};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             e[k] = exp2_approx(s[a][k] - (st.m[a][k & 1] == -INFINITY ? 0.0f : st.m[a][k & 1]));
             st.l[a][k & 1] += e[k];
-            e[k] *= w;
+            e[k] *= w[k & 1];
         }
         const uint32_t h0 = pack_half(e[0], e[1]), h1 = pack_half(e[2], e[3]);
         p[a][0] = make_uint2(transpose8x8(h0), transpose8x8(h1));
@@ -483,16 +475,17 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
             }
         constexpr uint32_t kPitch = D + 4;   // rows 4 banks apart: conflict-free 16-byte stores
         float *mo = reinterpret_cast<float *>(ring);
-        const float back = st.ref * (1.0f / kWeightScale);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j)
+            for (int r = 0; r < 2; ++r) {
+                const float back = back_of(st.m[n][r], st.mo[n][r]);
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
+                for (int j = 0; j < D / 32; ++j)
                     *reinterpret_cast<float4 *>(mo + (n * 8 + (lane & 3) * 2 + r) * kPitch + j * 32 + (lane >> 2) * 4) =
                         make_float4(st.o[n][2 * j][r] * back, st.o[n][2 * j][2 + r] * back, st.o[n][2 * j + 1][r] * back,
                                     st.o[n][2 * j + 1][2 + r] * back);
+            }
         __syncthreads();
         const bool begun = u0 == 0, ended = u1 == depth;
         const uint64_t place = 2ull * share + (begun ? 1 : 0);   // of a partial

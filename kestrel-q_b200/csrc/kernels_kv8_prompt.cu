@@ -281,7 +281,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.q_full);
 
-        float mx = -INFINITY, sum = 0.0f, ref = 0.0f;
+        float mx = -INFINITY, mo = -INFINITY, sum = 0.0f;   // mo: the reference point of O (kernels_kv8.cuh)
         const uint32_t o_at = tmem + lanes + m * D;
         const bool whole = groups <= each;
         const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, T::rows, D,
@@ -367,12 +367,13 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 id = page_of(j + 2);
                 const uint32_t s_at = tmem + lanes + T::s_col + m * T::tile_cols, p_at = T::alias ? s_at : s_at + T::tokens + (j & 1) * T::p_cols;
                 const int32_t token = (int32_t)((g0 + j * T::groups) * kG);
-                float f[T::groups], w[T::groups], most = 0.0f;
+                const float size = size_of(sc.y);
+                float f[T::groups], w[T::groups], lw[T::groups];
 #pragma unroll
                 for (uint32_t g = 0; g < T::groups; ++g) {
                     f[g] = factor * __shfl_sync(~0u, sc.x, g);
                     w[g] = __shfl_sync(~0u, sc.y, g);
-                    most = fmaxf(most, w[g]);
+                    lw[g] = __shfl_sync(~0u, size, g);
                 }
                 ok = bar_wait_warp(&sh.s_full[m], j & 1, quit);
                 if (!ok) break;
@@ -394,7 +395,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     for (int k = 0; k < (int)T::tokens; ++k)
                         if (k > seen) r[k / 32][k % 32] = 0xff800000u;
                 }
-                float top = -INFINITY;
+                float top = -INFINITY, top_o = -INFINITY;
                 {
                     float x[T::groups];
 #pragma unroll
@@ -409,22 +410,22 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                         // a factor of 0 (a zero page) would make -inf NaN
                         if (f[g] == 0.0f) f[g] = 1.0e-38f;
                         top = fmaxf(top, x[g] * f[g]);
+                        top_o = fmaxf(top_o, x[g] * f[g] + lw[g]);
                     }
                 }
                 float by = 1.0f;
                 if (top > mx + kRaise) {   // -inf + 8 is -inf: the first finite logit lifts
-                    by = exp2_approx(mx - top);
-                    mx = top;
-                    sum *= by;
-                    kept *= by;
+                    const float m_new = ceilf(top), l_by = exp2_approx(mx - m_new);
+                    mx = m_new;
+                    sum *= l_by;
+                    kept *= l_by;
                 }
-                if (most > ref) {
-                    // the next power of two, within the normal range
-                    const uint32_t e = min((__float_as_uint(most) + 0x7fffffu) & 0x7f800000u, 0x7f000000u);
-                    const float up = __uint_as_float(max(e, 0x00800000u));
-                    by *= ref / up;
-                    ref = up;
+                if (top_o > mo + kRaise) {
+                    const float m_new = ceilf(top_o);
+                    by = exp2_approx(mo - m_new);
+                    mo = m_new;
                 }
+                const float back = back_of(mx, mo);
                 const bool flush = TERMS == 2 && j > 0 && j % T::flush == 0;
                 // O is at rest once the last step's second product is done.  Every
                 // step waits for it before it hands its weights over, if not
@@ -437,7 +438,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     fence_after();
                     if (flush) {
                         // by: since the accumulators' scale; kept: since the saved sums'
-                        if constexpr (TERMS == 2) save(by * ref * (1.0f / kWeightScale), saved ? kept : 0.0f, false);
+                        if constexpr (TERMS == 2) save(by * back, saved ? kept : 0.0f, false);
                         saved = true;
                         kept = 1.0f;
                     } else {
@@ -453,7 +454,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     }
                 }
                 // weights
-                const float base = mx == -INFINITY ? 0.0f : mx, inv = ref > 0.0f ? kWeightScale / ref : 0.0f;
+                const float base = mx == -INFINITY ? 0.0f : mx, inv = weight_of(mx, mo);
                 const uint64_t base2 = pack2(-base, -base);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -497,7 +498,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             }
             if (ok && steps > 0) ok = bar_wait_warp(&pv_done[m], (steps - 1) & 1, quit);
             fence_after();
-            float scale = ref * (1.0f / kWeightScale);
+            float scale = back_of(mx, mo);
             if (TERMS == 2 && ok && saved) {
                 // the saved sums come back into TMEM before any row is final
                 save(scale, kept, true);

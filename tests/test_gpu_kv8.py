@@ -517,6 +517,40 @@ def test_attention_over_pages_of_different_size(kq, fmt):
         s.attend(step, new, 3, q=q)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("new", [1, 300])
+def test_attention_past_large_values(kq, dtype, dim, new):
+    """Pages of values 1e8 times the others', whose logits are 80 below: they
+    weigh nothing (1e8 e^-80), and the others keep their bits.  The bounds of
+    this file with W = sum p |v| in place of the largest value: errors are
+    relative to each weight.  (Weights of 22 bits below the largest value
+    alone would be wrong by 2^-5 here.)"""
+    s = Server(kq, 1, dim, 16, "int8", 1, 210, pages=70, dtype=dtype)
+    n, G = 700, 3
+    far = np.zeros(n, bool)
+    far[64:96] = far[304:320] = far[656:672] = True     # whole pages
+    k = (0.1 * s.rng.standard_normal((n, 1, dim))).astype(np.float32)
+    k[far] = 0
+    k[far, 0, 0] = -20
+    v = (s.rng.standard_normal((n, 1, dim)) * np.where(far, 1e8, 1)[:, None, None]).astype(np.float32)
+    s.step([n], k=k, v=v)
+    step = s.step([new], k=k[:1].repeat(new, 0), v=v[:1].repeat(new, 0))
+    q = s.rng.standard_normal((new, G, dim)).astype(np.float32)
+    q[:, :, 0] = 4
+    with Launches(kq, "kv8_prompt") as seen:
+        got, _ = s.attend(step, [new], G, scale=1.0, q=q, check=False)
+    assert seen.count == (new > 1)
+    if dtype == "bfloat16":
+        q = dev(q, dtype).float().cpu().numpy()
+    o, l, size, _ = ref.attend(s.ref, s.table, [n], [new], q, 1.0)
+    s.ref.code[:, :, 1] = np.abs(s.ref.code[:, :, 1])
+    w = ref.attend(s.ref, s.table, [n], [new], q, 1.0)[0].max(-1)
+    bo, _ = bounds(dtype, dim, n + new, size, w, o, l)
+    assert np.all(w < 10)
+    assert np.all(np.abs(got - o) <= bo), np.max(np.abs(got - o) / bo)
+
+
 def test_attention_twice_is_the_same(kq):
     s = Server(kq, 2, 128, 32, "int8", 2, 100)
     s.step([3000, 50])
