@@ -709,7 +709,9 @@ kq_status kq_b200_kv8_attend_workspace_bytes(const kq_b200_kv8_cache *cache,
  * nothing gets zeros and -infinity; rows behind the last request are left as
  * they were.  Uses step->block_table, query_offsets and kv_lengths only.
  * Query and output have the same type; products are exact in the codes and
- * hold 22 bits of an F32 query, sums and the softmax are F32.
+ * hold 22 bits of an F32 query, sums and the softmax are F32.  Weights are not
+ * normalised before they are summed: values of 2^100 and more can leave F32's
+ * range in long sums, which is reported like other non-finite values.
  * `max_kv_length` (0: what the table's columns hold) and the capacities only
  * decide how the work is cut; the result is right for any lengths, and the
  * same for the same cut.  `workspace` is private to the call until it has

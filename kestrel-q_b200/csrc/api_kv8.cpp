@@ -299,7 +299,8 @@ kq_status kq_b200_kv8_attend(const kq_b200_kv8_cache *cache, const kq_b200_kv8_s
         st = check_attend(c, s, query_heads, dtype == KQ_B200_KV8_BF16, max_kv_length, &shape, diagnostic);
     if (st != KQ_STATUS_OK) return st;
     if (!known_dtype(dtype)) return fail(diagnostic, KQ_STATUS_UNSUPPORTED_TENSOR_TYPE, "queries are F32 or BF16");
-    if (!std::isfinite(softmax_scale)) return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "softmax scale must be finite");
+    const float scale_log2 = softmax_scale * 1.44269504088896340736f;
+    if (!std::isfinite(scale_log2)) return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "softmax scale must be finite");
     const uint32_t size = dtype == KQ_B200_KV8_F32 ? 4 : 2;
     const uint64_t width = (uint64_t)query_heads * c.dim, B = s.requests;
     uint64_t qb, ob;
@@ -325,7 +326,7 @@ kq_status kq_b200_kv8_attend(const kq_b200_kv8_cache *cache, const kq_b200_kv8_s
     if (st != KQ_STATUS_OK) return st;
     std::lock_guard<std::recursive_mutex> lk(ctx->mu);
     const Kv8Attend a{query, output, lse, query_stride, output_stride, query_heads, dtype == KQ_B200_KV8_BF16,
-                      softmax_scale * 1.44269504088896340736f, static_cast<float *>(workspace)};
+                      scale_log2, static_cast<float *>(workspace)};
     launch_kv8_attend(c, s, a, shape, ctx->begin_call(), ctx->stream);
     KQB_CUDA(cudaGetLastError(), diagnostic, "cache attention launch");
     return KQ_STATUS_OK;

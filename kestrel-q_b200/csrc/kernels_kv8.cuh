@@ -14,7 +14,8 @@ namespace {
 constexpr uint32_t kG = kKv8GroupTokens;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kRaise = 8.0f;        // a logit this far above its reference point raises that
-constexpr float kWeightScale = 64.0f; // 2^6
+constexpr float kWeightBits = 6.0f;
+constexpr float kMost = 3.40282347e38f;
 constexpr uint32_t kTryNs = 100000;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kPromptUnit = 8;   // groups: a prompt's split is whole steps of 128 tokens
@@ -119,20 +120,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// A row's two reference points, both whole numbers, so that every factor made
-// of them is an exact power of two.  m: logits, for the sum l.  mo: logits plus
-// log2 of the page's value scale, for O: a weight enters the second product as
-//   p sV 2^(m - mo) 2^6,   p = 2^(l - m)
+// A row's two reference points, whole numbers, so that every factor made of
+// them is an exact power of two: m for logits and the sum l, m + z for O, whose
+// weights have the page's value scale in them.  A weight enters the second
+// product as
+//   p sV 2^(6 - z),   p = 2^(l - m)
 // at most 2^14; it loses bits only where it is small beside the row's largest
-// p sV, however large the values that the row does not attend to.  Scales below
-// 2^-110 count as that, which bounds m - mo (both move when they are 8 below a
-// step's largest).
-__device__ __forceinline__ float size_of(float scale) { return fmaxf(__log2f(scale), -110.0f); }
-__device__ __forceinline__ float weight_of(float m, float mo) {   // of sV p
-    return m == -INFINITY ? 0.0f : exp2_approx(m - mo) * kWeightScale;
+// p sV, however large the values that the row does not attend to.  Either point
+// moves when it is 8 below a step's largest.  Scales below 2^-80 count as that,
+// which bounds z from below; sV 2^(6 - z) can only overflow (scales from 2^33,
+// beside such small ones) where p is below 2^-114, and stays finite then.
+__device__ __forceinline__ float size_of(float scale) { return fmaxf(__log2f(scale), -80.0f); }
+__device__ __forceinline__ float weight_of(float m, float z) {   // of p sV
+    return m == -INFINITY ? 0.0f : exp2_approx(kWeightBits - z);
 }
-__device__ __forceinline__ float back_of(float m, float mo) {   // of O, to units of 2^m
-    return m == -INFINITY ? 0.0f : exp2_approx(mo - m) * (1.0f / kWeightScale);
+__device__ __forceinline__ float back_of(float m, float z) {   // of O, to units of 2^m
+    return m == -INFINITY ? 0.0f : exp2_approx(z - kWeightBits);
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {

@@ -126,13 +126,13 @@ constexpr uint32_t kRowSmem = kRowWarps * kRowStages<D, NT> * 32 * D + NT * TERM
 template <int D, int NT>
 struct Columns {
     float o[NT][D / 16][4];
-    float m[NT][2], mo[NT][2], l[NT][2];
+    float m[NT][2], z[NT][2], l[NT][2];   // reference points m, m + z; sums
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) m[a][r] = mo[a][r] = -INFINITY, l[a][r] = 0.0f;
+            for (int r = 0; r < 2; ++r) m[a][r] = z[a][r] = -INFINITY, l[a][r] = 0.0f;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
 #pragma unroll
@@ -202,7 +202,7 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
             top[a][r] = x;
-            lift |= x > st.m[a][r] + kRaise || x + size > st.mo[a][r] + kRaise;
+            lift |= x > st.m[a][r] + kRaise || x - st.m[a][r] + size > st.z[a][r] + kRaise;
         }
     }
     if (__any_sync(~0u, lift)) {   // -inf + 8 is -inf: the first finite logit of a row lifts it
@@ -211,15 +211,14 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
             float by[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float m = fmaxf(st.m[a][r], ceilf(top[a][r])), mo = fmaxf(st.mo[a][r], ceilf(top[a][r] + size));
-                if (m == -INFINITY) {
-                    by[r] = 1.0f;
-                    continue;
-                }
-                st.l[a][r] *= exp2_approx(st.m[a][r] - m);
-                by[r] = exp2_approx(st.mo[a][r] - mo);
+                const float m = fmaxf(st.m[a][r], ceilf(top[a][r]));
+                by[r] = 1.0f;
+                if (m == -INFINITY) continue;
+                const float less = st.m[a][r] - m, old = st.z[a][r] + less, z = fmaxf(old, ceilf(top[a][r] - m + size));
+                st.l[a][r] *= exp2_approx(less);
+                by[r] = exp2_approx(old - z);
                 st.m[a][r] = m;
-                st.mo[a][r] = mo;
+                st.z[a][r] = z;
             }
 #pragma unroll
             for (int n = 0; n < D / 16; ++n)
@@ -231,7 +230,7 @@ __device__ __forceinline__ void column_step(Columns<D, NT> &st, const uint2 *q, 
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
         float e[4];
-        const float w[2] = {weight_of(st.m[a][0], st.mo[a][0]) * vs, weight_of(st.m[a][1], st.mo[a][1]) * vs};
+        const float w[2] = {fminf(weight_of(st.m[a][0], st.z[a][0]) * vs, kMost), fminf(weight_of(st.m[a][1], st.z[a][1]) * vs, kMost)};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             e[k] = exp2_approx(s[a][k] - (st.m[a][k & 1] == -INFINITY ? 0.0f : st.m[a][k & 1]));
@@ -479,7 +478,7 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float back = back_of(st.m[n][r], st.mo[n][r]);
+                const float back = back_of(st.m[n][r], st.z[n][r]);
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j)
                     *reinterpret_cast<float4 *>(mo + (n * 8 + (lane & 3) * 2 + r) * kPitch + j * 32 + (lane >> 2) * 4) =

@@ -281,7 +281,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         __syncwarp();
         if (lane == 0) bar_arrive(&sh.q_full);
 
-        float mx = -INFINITY, mo = -INFINITY, sum = 0.0f;   // mo: the reference point of O (kernels_kv8.cuh)
+        float mx = -INFINITY, z = -INFINITY, sum = 0.0f;   // reference points: mx of logits, mx + z of O
         const uint32_t o_at = tmem + lanes + m * D;
         const bool whole = groups <= each;
         const Partials part(a.workspace + shape.row_floats, (uint64_t)t * c.heads + head, shape.prompt_splits, T::rows, D,
@@ -302,7 +302,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
         // bytes of the rows one after another, so that a warp writes 512
         // contiguous bytes; in a tile's rest, in its row.
         bool saved = false;
-        float kept = 1.0f;      // what the saved sums are to be multiplied by
+        float kept = 1.0f;      // what the saved sums are to be multiplied by (they are in O's unit, far from overflow)
         const bool full_tile = row0 + m * 128 + 128 <= row_end;
         auto save = [&](float scale, float keep, bool final_to_tmem) {
             constexpr uint32_t Q = D / 4, kRowsOn = 128 / Q;   // pieces in a row; rows from piece f to piece f + 1 of a thread
@@ -395,37 +395,48 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     for (int k = 0; k < (int)T::tokens; ++k)
                         if (k > seen) r[k / 32][k % 32] = 0xff800000u;
                 }
-                float top = -INFINITY, top_o = -INFINITY;
-                {
-                    float x[T::groups];
+                float top = -INFINITY, high[T::groups];
 #pragma unroll
-                    for (uint32_t g = 0; g < T::groups; ++g) x[g] = -INFINITY;
+                for (uint32_t g = 0; g < T::groups; ++g) high[g] = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 16; k += 2)
+                for (int k = 0; k < 16; k += 2)
 #pragma unroll
-                        for (uint32_t g = 0; g < T::groups; ++g)
-                            x[g] = max3(x[g], __uint_as_float(r[g / 2][g % 2 * 16 + k]), __uint_as_float(r[g / 2][g % 2 * 16 + k + 1]));
+                    for (uint32_t g = 0; g < T::groups; ++g)
+                        high[g] = max3(high[g], __uint_as_float(r[g / 2][g % 2 * 16 + k]), __uint_as_float(r[g / 2][g % 2 * 16 + k + 1]));
 #pragma unroll
-                    for (uint32_t g = 0; g < T::groups; ++g) {
-                        // a factor of 0 (a zero page) would make -inf NaN
-                        if (f[g] == 0.0f) f[g] = 1.0e-38f;
-                        top = fmaxf(top, x[g] * f[g]);
-                        top_o = fmaxf(top_o, x[g] * f[g] + lw[g]);
-                    }
+                for (uint32_t g = 0; g < T::groups; ++g) {
+                    // a factor of 0 (a zero page) would make -inf NaN
+                    if (f[g] == 0.0f) f[g] = 1.0e-38f;
+                    high[g] *= f[g];
+                    top = fmaxf(top, high[g]);
+                }
+                // The weights' exponents come from one fused multiply and add each,
+                // whose product is not rounded as `top` is: a difference that
+                // counts from logits of 2^24 on.  There the products are rounded
+                // first.
+                if (__any_sync(~0u, fabsf(top) > 0x1p20f && top > -INFINITY)) {
+                    asm volatile("");   // a branch
+#pragma unroll
+                    for (uint32_t k = 0; k < T::tokens; ++k) r[k / 32][k % 32] = __float_as_uint(__uint_as_float(r[k / 32][k % 32]) * f[k / 16]);
+#pragma unroll
+                    for (uint32_t g = 0; g < T::groups; ++g) f[g] = 1.0f;
                 }
                 float by = 1.0f;
                 if (top > mx + kRaise) {   // -inf + 8 is -inf: the first finite logit lifts
-                    const float m_new = ceilf(top), l_by = exp2_approx(mx - m_new);
-                    mx = m_new;
+                    const float to = ceilf(top), less = mx - to, l_by = exp2_approx(less);
+                    mx = to;
+                    z += less;
                     sum *= l_by;
-                    kept *= l_by;
                 }
-                if (top_o > mo + kRaise) {
-                    const float m_new = ceilf(top_o);
-                    by = exp2_approx(mo - m_new);
-                    mo = m_new;
+                float top_o = -INFINITY;   // (a row that has seen nothing: NaNs, which the maximum drops)
+#pragma unroll
+                for (uint32_t g = 0; g < T::groups; ++g) top_o = fmaxf(top_o, high[g] - mx + lw[g]);
+                if (top_o > z + kRaise) {
+                    const float to = ceilf(top_o);
+                    by = exp2_approx(z - to);
+                    kept *= by;
+                    z = to;
                 }
-                const float back = back_of(mx, mo);
                 const bool flush = TERMS == 2 && j > 0 && j % T::flush == 0;
                 // O is at rest once the last step's second product is done.  Every
                 // step waits for it before it hands its weights over, if not
@@ -437,8 +448,8 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     if (!ok) break;
                     fence_after();
                     if (flush) {
-                        // by: since the accumulators' scale; kept: since the saved sums'
-                        if constexpr (TERMS == 2) save(by * back, saved ? kept : 0.0f, false);
+                        // by: since the accumulators' reference point; kept: since the saved sums'
+                        if constexpr (TERMS == 2) save(by, saved ? kept : 0.0f, false);
                         saved = true;
                         kept = 1.0f;
                     } else {
@@ -454,7 +465,9 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     }
                 }
                 // weights
-                const float base = mx == -INFINITY ? 0.0f : mx, inv = weight_of(mx, mo);
+                const float base = mx == -INFINITY ? 0.0f : mx, inv = weight_of(mx, z);
+#pragma unroll
+                for (uint32_t g = 0; g < T::groups; ++g) w[g] = fminf(w[g] * inv, kMost);
                 const uint64_t base2 = pack2(-base, -base);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -477,7 +490,7 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                         const int at = (k >> 3) * 16 + (k & 1) * 8 + (k >> 1 & 3) * 2;
                         const uint64_t e2 = pack2(__uint_as_float(r[q][at]), __uint_as_float(r[q][at + 1]));
                         sum2[k & 1] = add2(sum2[k & 1], e2);
-                        const float v = w[2 * q + (k >> 3)] * inv;
+                        const float v = w[2 * q + (k >> 3)];
                         float x, y;
                         unpack2(mul2(e2, pack2(v, v)), x, y);
                         hi[k] = pack_half(x, y);
@@ -498,11 +511,10 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
             }
             if (ok && steps > 0) ok = bar_wait_warp(&pv_done[m], (steps - 1) & 1, quit);
             fence_after();
-            float scale = back_of(mx, mo);
+            float scale = back_of(mx, z);
             if (TERMS == 2 && ok && saved) {
                 // the saved sums come back into TMEM before any row is final
-                save(scale, kept, true);
-                scale = 1.0f;
+                save(1.0f, kept, true);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.back[m]);

@@ -551,6 +551,40 @@ def test_attention_past_large_values(kq, dtype, dim, new):
     assert np.all(np.abs(got - o) <= bo), np.max(np.abs(got - o) / bo)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new", [1, 300])
+@pytest.mark.parametrize("value,logit", [(1e9, 1e12), (1e-7, 3e10), (1e36, 5.0), (3e-24, 5.0), (1e30, 1e-20)])
+def test_attention_of_large_logits_and_values(kq, dtype, new, value, logit):
+    """Logits up to 1e12, where one token wins, with values of many sizes; the
+    largest and the smallest values that the reference points allow."""
+    s = Server(kq, 1, 64, 16, "int8", 1, 210, pages=70, dtype=dtype, seed=3)
+    n, G = 500, 3
+    k = s.rng.standard_normal((n + new, 1, 64)).astype(np.float32)
+    v = (value * s.rng.standard_normal((n + new, 1, 64))).astype(np.float32)
+    s.step([n], k=k[:n], v=v[:n])
+    step = s.step([new], k=k[n:], v=v[n:])
+    q = (logit * s.rng.standard_normal((new, G, 64))).astype(np.float32)
+    got, _ = s.attend(step, [new], G, scale=1.0, q=q, check=False)
+    q = dev(q, dtype).float().cpu().numpy()
+    o, l, size, _ = ref.attend(s.ref, s.table, [n], [new], q, 1.0)
+    s.ref.code[:, :, 1] = np.abs(s.ref.code[:, :, 1])
+    w = ref.attend(s.ref, s.table, [n], [new], q, 1.0)[0].max(-1)
+    assert np.all(np.isfinite(got))
+    if logit > 1e3:
+        # rows whose winner stands out by more than the logits' errors (times 2 for a pair, and 100 to be e^-100 behind)
+        kv = s.ref.rows(s.table[0], n + new)[0, 0]
+        x = q.astype(np.float64) @ kv.T
+        x[np.arange(n + new) > n + np.arange(new)[:, None, None].repeat(G, 1)] = -np.inf
+        x.sort(-1)
+        clear = x[..., -1] - x[..., -2] > 100 + 4 * size * (8 + 64 / 4) * U
+        assert clear.mean() > 0.8
+        step = 2.0 ** -8 + 2.0 ** -11 if dtype == "bfloat16" else 2.0 ** -20
+        assert np.all(np.abs(got - o)[clear] <= (step * np.abs(o) + 2.0 ** -20 * w[..., None])[clear])
+    else:
+        bo, _ = bounds(dtype, 64, n + new, size, w, o, l)
+        assert np.all(np.abs(got - o) <= bo), np.max(np.abs(got - o) / bo)
+
+
 def test_attention_twice_is_the_same(kq):
     s = Server(kq, 2, 128, 32, "int8", 2, 100)
     s.step([3000, 50])

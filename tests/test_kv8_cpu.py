@@ -135,7 +135,7 @@ def test_refused_attention(kq):
     assert attend(kq, dtype=7) == a.UNSUPPORTED_TENSOR_TYPE
     for heads in (0, 7, 3):
         assert attend(kq, heads=heads) == a.DIMENSION_MISMATCH
-    for scale in (math.nan, math.inf, -math.inf):
+    for scale in (math.nan, math.inf, -math.inf, 3e38):   # the last: not finite in base 2
         assert attend(kq, scale=scale) == a.INVALID_ARGUMENT
     for name in ("q", "out"):
         assert attend(kq, **{name: None}) == a.INVALID_ARGUMENT
