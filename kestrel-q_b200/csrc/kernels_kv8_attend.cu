@@ -299,9 +299,9 @@ struct ShareSpace {
 // tile through its own ring; page ids and scales of its next 64 groups sit in
 // its lanes.
 // Measured: 64 F32 sequences, contexts U[1k, 32k], 16 heads of 256 over int8
-// pages: 1086 MB in 191 us with the join (5.7 TB/s of the measured 6.5; under
-// ncu the kernel alone 173 us); 96 bf16 sequences up to 8k, 32 heads of 128 over
-// e4m3 pages: 892 MB in 162 us.  (16 rows on the M side, one split per 2048
+// pages: 1086 MB in 191 to 203 us, by machine, with the join (5.7 to 5.3 TB/s of the
+// measured 6.5; under ncu the kernel alone 173 to 180 us); 96 bf16 sequences up to 8k, 32 heads of 128 over
+// e4m3 pages: 892 MB in 160 to 166 us.  (16 rows on the M side, one split per 2048
 // tokens and a join kernel per row: 244 and 242 us.)
 template <int D, int NT, int TERMS, bool E4M3>
 __global__ void __launch_bounds__(kRowThreads, (kRowCtas<D, NT>))

@@ -24,7 +24,7 @@
 //
 // Bound: the chain softmax -> second product -> first product of a tile; the
 // tensor pipe is busy a third of the time.  Measured: an 8k bf16 prompt, 32
-// query heads of 128 over int8 pages, 836 us: 658 TFLOP/s of the measured 1662
+// query heads of 128 over int8 pages, 843 us: 652 TFLOP/s of the measured 1662
 // (mma.sync tiles: 1843 us); of a step's 6200 cycles a tile spends 3700 in its
 // softmax (2000 of them on the weights' exponentials, which both tiles share
 // one unit for) and 1900 waiting for its two products.  F32 (two-term operands:
