@@ -654,6 +654,7 @@ class Kv8Cache:
         return dtype, a.data_ptr(), stride[0] if tokens > 1 else shape[1] * d
 
     def plan(self, step: Kv8Step, context_lengths, new_lengths, free_pages, free_head, free_head_out) -> None:
+        """Fills `step` from the requests' cached and new lengths; pages come from free_pages[free_head[0]:]."""
         n = step.args.request_count
         for a, least in ((context_lengths, n), (new_lengths, n), (free_pages, 0), (free_head, 1), (free_head_out, 1)):
             if a.dtype != self._int32 or a.numel() < least or not a.is_contiguous():
@@ -664,6 +665,7 @@ class Kv8Cache:
                                          free_head_out.data_ptr(), C.byref(d)), d)
 
     def append(self, step: Kv8Step, key, value) -> None:
+        """Quantises `key` and `value` [tokens][kv heads][head_dim] (float32 or bfloat16) into the step's slots."""
         n = step.args.token_capacity
         kt, kp, ks = self._rows("key", key, n, self.kv_heads)
         vt, vp, vs = self._rows("value", value, n, self.kv_heads)

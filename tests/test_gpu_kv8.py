@@ -253,6 +253,31 @@ def test_append_of_special_rows(kq, fmt):
     s.check_pages()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("size", [1.0, 0.3, 1 / 3, 1.1e-20, 7e8, 2e-36, 3e33])
+def test_append_at_the_rounding_borders(kq, fmt, size):
+    """Every border between two codes, and the F32 values up to three steps
+    from it, times the page's scale: quotients that a product with a rounded
+    reciprocal would put on the other side."""
+    s = Server(kq, 1, 256, 16, fmt, 1, 1)
+    most = ref.LARGEST[fmt]
+    codes = np.arange(-127, 128) if fmt == "int8" else np.unique(ref.E4M3[np.isfinite(ref.E4M3)])
+    border = ((codes[1:].astype(np.float64) + codes[:-1]) / 2)
+    x = (border * size).astype(np.float32)
+    near = [x]
+    for to in (np.float32(-np.inf), np.float32(np.inf)):
+        y = x
+        for _ in range(3):
+            near.append(y := np.nextafter(y, to))
+    near = np.concatenate(near)
+    rows = np.zeros((2, 16 * 256), np.float32)
+    rows[:, 1:1 + near.size] = near
+    rows[:, 0] = np.float32(most * size)     # the scale: this / most, about `size`
+    rows[1] = -rows[1]
+    s.step([16], k=rows[0].reshape(16, 1, 256), v=rows[1].reshape(16, 1, 256))
+    s.check_pages()
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_append_of_non_finite_rows(kq, value):
     """Reported, and the (page, head, side) keeps what it held."""
