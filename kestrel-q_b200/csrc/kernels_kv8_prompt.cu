@@ -413,7 +413,8 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 // The weights' exponents come from one fused multiply and add each,
                 // whose product is not rounded as `top` is: a difference that
                 // counts from logits of 2^24 on.  There the products are rounded
-                // first.
+                // first.  (The branch takes 12 us of an 8k bf16 prompt's 839; behind
+                // the lifts, with the products divided by their factors, 25.)
                 if (__any_sync(~0u, fabsf(top) > 0x1p20f && top > -INFINITY)) {
                     asm volatile("");   // a branch
 #pragma unroll
