@@ -107,10 +107,13 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
 
 // The same for a whole warp, with the same answer in every lane; one lane
 // polls (polls are shared-memory traffic: with all lanes the row kernel took
-// 203 us for 64 F32 sequences, not 192).
+// 203 us for 64 F32 sequences, not 192).  What that lane's wait acquired is
+// ordered before the other lanes' accesses by the warp barrier; a shuffle
+// orders no memory.
 __device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, volatile uint32_t *quit = nullptr) {
     uint32_t ok = 0;
     if ((threadIdx.x & 31) == 0) ok = bar_wait(bar, parity, quit);
+    __syncwarp();
     return __shfl_sync(~0u, ok, 0) != 0;
 }
 
