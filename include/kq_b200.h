@@ -432,7 +432,8 @@ kq_status kq_b200_layer_config_bind(kq_layer_config *config,
 /* Selects the device used by subsequently created objects (default 0). */
 kq_status kq_b200_set_device(int device, kq_diagnostic *diagnostic);
 /* Replaces the library's stream on the current device (cudaStream_t, or
- * NULL to restore the library's own non-blocking stream). */
+ * NULL to restore the library's own non-blocking stream; the legacy default
+ * stream is cudaStreamLegacy), after waiting for the old one. */
 kq_status kq_b200_set_stream(void *cuda_stream, kq_diagnostic *diagnostic);
 void *kq_b200_get_stream(void);
 

@@ -17,7 +17,7 @@ from . import abi, synth
 from .abi import KQError, lib
 
 __all__ = ["abi", "synth", "lib", "KQError", "Provider", "GdnLayer", "GdnState", "QsaLayer",
-           "QsaState", "Kv8Cache", "Kv8Step", "build"]
+           "QsaState", "Kv8Cache", "Kv8Step", "set_stream", "build"]
 
 
 def build(force: bool = False):
@@ -578,6 +578,31 @@ def qsa_prefill_sharded_async(state: QsaState, x_ptr: int, tokens: int, y_ptr: i
                                                     world, token_part, token_parts, exchange, None, C.byref(d)), d)
 
 
+def set_stream(stream=None) -> None:
+    """Makes a torch stream the library stream of the current device; None: the library's own."""
+    d = abi.Diagnostic()
+    # torch's default stream has handle 0, which the library takes for its own: 1 is CUDA's name for it
+    abi.check(lib().kq_b200_set_stream(None if stream is None else stream.cuda_stream or 1, C.byref(d)), d)
+
+
+def _in_order(device, call, *args) -> None:
+    """`call` in the order of torch's current stream on `device`: after what
+    that stream holds, and before what it is given next (so memory that torch
+    reuses on it is no longer in use).  Two events, unless it is the library
+    stream (:func:`set_stream`)."""
+    import torch
+    here, handle = torch.cuda.current_stream(device), lib().kq_b200_get_stream()
+    d = abi.Diagnostic()
+    if (here.cuda_stream or 1) == handle:
+        abi.check(call(*args, C.byref(d)), d)
+        return
+    library = torch.cuda.ExternalStream(handle)   # get_stream leaves the library's device current
+    library.wait_stream(here)
+    status = call(*args, C.byref(d))
+    here.wait_stream(library)
+    abi.check(status, d)
+
+
 class Kv8Step:
     """The device arrays of one step of a paged cache (kq_b200_kv8_step):
     `requests` rows of `block_table` (int32 [requests][columns], the caller's),
@@ -616,7 +641,9 @@ class Kv8Step:
 class Kv8Cache:
     """A paged 8-bit key/value cache (kq_b200_kv8_cache) over torch arrays:
     `codes` (uint8) and `scales` (float32), allocated empty if not given.
-    The calls are asynchronous on the library stream."""
+    The calls run on the library stream, asynchronously, in the order of torch's
+    current stream like torch's own operations: arrays made on another stream,
+    or freed there, are the caller's to order (wait_stream, record_stream)."""
 
     FORMATS = {"int8": 0, "e4m3": 1}
 
@@ -659,10 +686,9 @@ class Kv8Cache:
         for a, least in ((context_lengths, n), (new_lengths, n), (free_pages, 0), (free_head, 1), (free_head_out, 1)):
             if a.dtype != self._int32 or a.numel() < least or not a.is_contiguous():
                 raise ValueError("a plan takes consecutive int32 lengths, free pages and heads")
-        d = abi.Diagnostic()
-        abi.check(lib().kq_b200_kv8_plan(self.args, step.args, context_lengths.data_ptr(), new_lengths.data_ptr(),
-                                         free_pages.data_ptr(), free_pages.numel(), free_head.data_ptr(),
-                                         free_head_out.data_ptr(), C.byref(d)), d)
+        _in_order(self.codes.device, lib().kq_b200_kv8_plan, self.args, step.args, context_lengths.data_ptr(),
+                  new_lengths.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_head.data_ptr(),
+                  free_head_out.data_ptr())
 
     def append(self, step: Kv8Step, key, value) -> None:
         """Quantises `key` and `value` [tokens][kv heads][head_dim] (float32 or bfloat16) into the step's slots."""
@@ -671,16 +697,14 @@ class Kv8Cache:
         vt, vp, vs = self._rows("value", value, n, self.kv_heads)
         if kt != vt:
             raise ValueError("key and value must have the same type")
-        d = abi.Diagnostic()
-        abi.check(lib().kq_b200_kv8_append(self.args, step.args, kt, kp, ks, vp, vs, C.byref(d)), d)
+        _in_order(self.codes.device, lib().kq_b200_kv8_append, self.args, step.args, kt, kp, ks, vp, vs)
 
     def read_pages(self, pages, values) -> None:
         """values (float32 [pages][heads][key, value][page_tokens][head_dim]) of the page ids `pages` (int32)."""
         if pages.dtype != self._int32 or values.dtype != self._float32 or not (pages.is_contiguous() and values.is_contiguous()):
             raise ValueError("contiguous int32 pages and float32 values are required")
-        d = abi.Diagnostic()
-        abi.check(lib().kq_b200_kv8_read(self.args, pages.data_ptr(), pages.numel(), values.data_ptr(), values.numel(),
-                                         C.byref(d)), d)
+        _in_order(self.codes.device, lib().kq_b200_kv8_read, self.args, pages.data_ptr(), pages.numel(), values.data_ptr(),
+                  values.numel())
 
     def attend_workspace_bytes(self, step: Kv8Step, query_heads: int, max_kv_length: int = 0) -> int:
         n, d = C.c_uint64(), abi.Diagnostic()
@@ -703,11 +727,9 @@ class Kv8Cache:
                 raise ValueError("lse: one float32 per token and query head is required")
         if workspace is not None and not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        d = abi.Diagnostic()
-        abi.check(lib().kq_b200_kv8_attend(self.args, step.args, qt, qp, qs, query.shape[1], scale, max_kv_length, op, os,
-                                           None if lse is None else lse.data_ptr(),
-                                           None if workspace is None else workspace.data_ptr(),
-                                           0 if workspace is None else workspace.nbytes, C.byref(d)), d)
+        _in_order(self.codes.device, lib().kq_b200_kv8_attend, self.args, step.args, qt, qp, qs, query.shape[1], scale,
+                  max_kv_length, op, os, None if lse is None else lse.data_ptr(),
+                  None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes)
 
 
 def _tensor(name: str, a, dtype: str):
