@@ -324,6 +324,10 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
     if (tid < kRowWarps * ST) bar_init(&full[0][0] + tid, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pdl_wait();
+    // before any way out: the join reads every share's cut, and the error that
+    // ends this kernel may be cleared before the join looks (a graph's replay on
+    // one stream, a synchronize of another)
+    if (shares > 1 && tid == 0) space.cuts[share].last = 0;
     if (__syncthreads_or(tid == 0 && err_raised(err))) return;
 
     // units of all requests: consecutive requests per thread, then the request
@@ -352,7 +356,6 @@ kv8_rows_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord er
         if (w < (int)warp) upto += warp_units[w];
         total += warp_units[w];
     }
-    if (shares > 1 && tid == 0) space.cuts[share].last = 0;
     const uint32_t working = (uint32_t)min((uint64_t)shares, max(total / kMinShare, (uint64_t)1));
     if (share >= working || total == 0) return;
     uint64_t at = share_begin(total, share, working);

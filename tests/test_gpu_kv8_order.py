@@ -1,5 +1,7 @@
 """Paged 8-bit cache on the GPU: results that hang on the order of memory
 accesses, inside the kernels and between streams."""
+import math
+
 import numpy as np
 import pytest
 
@@ -113,3 +115,27 @@ def test_capture_of_torch_and_cache_together(kq):
         bo, _ = bounds("float32", 64, 901, size, top, o, l)
         assert np.all(np.abs(got - 1 - o) <= bo + (1 + np.abs(o)) * 2 * U)
     del graph
+
+
+def test_attention_after_an_error_leaves_no_cuts(kq):
+    """What a kernel that ends at once leaves in the workspace for the join:
+    cuts that say nothing was cut, not what the memory held (ones here)."""
+    import torch
+    s = Server(kq, 1, 64, 16, "int8", 2, 500)
+    s.step([50, 20])
+    step = s.step([1, 1])
+    q = torch.zeros(2, 4, 64, device="cuda")
+    out = torch.zeros_like(q)
+    nbytes = s.cache.attend_workspace_bytes(step, 4)
+    ws = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")
+    # floats of a share: two partials of 8 rows of (64 + 2), then a cut of four words, the last of them `last`
+    shares = nbytes // 4 // (2 * 8 * 66 + 4)
+    assert shares > 100
+    s.cache.append(step, torch.full((2, 1, 64), math.inf, device="cuda"), torch.zeros(2, 1, 64, device="cuda"))
+    s.cache.attend(step, q, out, scale=0.125, workspace=ws)
+    with pytest.raises(kq.KQError) as e:
+        kq.synchronize()
+    assert e.value.status == kq.abi.NUMERIC_DOMAIN
+    first = 2 * shares * 8 * 66
+    last = ws.view(torch.int32)[first:first + 4 * shares].view(shares, 4)[:, 3]
+    assert torch.all(last == 0)
