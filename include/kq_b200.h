@@ -436,6 +436,12 @@ kq_status kq_b200_set_device(int device, kq_diagnostic *diagnostic);
  * stream is cudaStreamLegacy), after waiting for the old one. */
 kq_status kq_b200_set_stream(void *cuda_stream, kq_diagnostic *diagnostic);
 void *kq_b200_get_stream(void);
+/* Orders what is enqueued from now on behind what is enqueued already, without
+ * waiting on the host: on the library stream behind `cuda_stream`, a stream of
+ * the current device (NULL: the legacy default stream), or with library_first
+ * the other way round.  Can be captured: the later stream joins the earlier
+ * one's capture. */
+kq_status kq_b200_order_stream(void *cuda_stream, int library_first, kq_diagnostic *diagnostic);
 
 /* One decode token for each of `batch` independent sequences.
  * `hidden` and `output` are device arrays [batch][hidden_size]; states are

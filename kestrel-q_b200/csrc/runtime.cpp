@@ -94,6 +94,8 @@ DeviceContext *context_for(int device) {
     if (cudaSetDevice(device) != cudaSuccess) return nullptr;
     if (cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking) != cudaSuccess) return nullptr;
     c->stream = c->own_stream;
+    for (cudaEvent_t &e : c->order)
+        if (cudaEventCreateWithFlags(&e, cudaEventDisableTiming) != cudaSuccess) return nullptr;
     if (cudaMalloc(&c->err_word, sizeof(unsigned long long)) != cudaSuccess) return nullptr;
     if (cudaMallocHost(&c->err_host, sizeof(unsigned long long)) != cudaSuccess) return nullptr;
     if (cudaMemset(c->err_word, 0, sizeof(unsigned long long)) != cudaSuccess) return nullptr;
@@ -352,6 +354,20 @@ void *kq_b200_get_stream(void) {
     DeviceContext *c;
     if (context(&c, nullptr) != KQ_STATUS_OK) return nullptr;
     return c->stream;
+}
+
+kq_status kq_b200_order_stream(void *cuda_stream, int library_first, kq_diagnostic *diagnostic) {
+    kq_diagnostic_clear(diagnostic);
+    DeviceContext *c;
+    kq_status st = context(&c, diagnostic);
+    if (st != KQ_STATUS_OK) return st;
+    std::lock_guard<std::recursive_mutex> lk(c->mu);
+    const cudaStream_t other = static_cast<cudaStream_t>(cuda_stream);
+    if (other == c->stream) return KQ_STATUS_OK;
+    const cudaEvent_t event = c->order[library_first != 0];
+    KQB_CUDA(cudaEventRecord(event, library_first ? c->stream : other), diagnostic, "stream order record");
+    KQB_CUDA(cudaStreamWaitEvent(library_first ? other : c->stream, event, 0), diagnostic, "stream order wait");
+    return KQ_STATUS_OK;
 }
 
 kq_status kq_b200_synchronize(kq_diagnostic *diagnostic) {

@@ -71,6 +71,7 @@ struct DeviceContext {
     int device = 0;
     cudaStream_t own_stream = nullptr;
     cudaStream_t stream = nullptr;
+    cudaEvent_t order[2] = {};                // of kq_b200_order_stream, by who goes first
     unsigned long long *err_word = nullptr;   // device
     unsigned long long *err_host = nullptr;   // pinned
     uint32_t next_call = 1;

@@ -239,6 +239,7 @@ _SIGNATURES = {
     "kq_b200_set_device": (C.c_int, [C.c_int, vp]),
     "kq_b200_set_stream": (C.c_int, [vp, vp]),
     "kq_b200_get_stream": (vp, []),
+    "kq_b200_order_stream": (C.c_int, [vp, C.c_int, vp]),
     "kq_b200_synchronize": (C.c_int, [vp]),
     "kq_b200_kernel_launch_count": (u64, []),
     "kq_b200_provider_create": (C.c_int, [C.c_int, C.POINTER(vp), vp]),

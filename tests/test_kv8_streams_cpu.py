@@ -17,6 +17,11 @@ class Library:
         self.log.append(("set", stream))
         return 0
 
+    def kq_b200_order_stream(self, stream, library_first, _):
+        first, then = (self.stream, stream) if library_first else (stream, self.stream)
+        self.log.append((then, "waits for", first))
+        return 0
+
     def __getattr__(self, name):
         if name in ("kq_b200_kv8_plan", "kq_b200_kv8_append", "kq_b200_kv8_read", "kq_b200_kv8_attend"):
             return lambda *_: self.log.append(("call", name)) or 0
@@ -24,11 +29,8 @@ class Library:
 
 
 class Stream:
-    def __init__(self, log, handle):
-        self.log, self.cuda_stream = log, handle
-
-    def wait_stream(self, other):
-        self.log.append((self.cuda_stream, "waits for", other.cuda_stream))
+    def __init__(self, handle):
+        self.cuda_stream = handle
 
 
 @pytest.mark.parametrize("torch_stream,library", [(0, 7), (5, 7), (7, 7), (0, 1)])
@@ -36,9 +38,9 @@ def test_calls_in_the_order_of_torch(kq, monkeypatch, torch_stream, library):
     log = []
     real = kq.lib()
     monkeypatch.setattr(kq, "lib", lambda: Library(real, log, library))
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(log, torch_stream))
-    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: Stream(log, handle))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: {3: torch_stream}[device], raising=False)
     cache = kq.Kv8Cache(1, 64, 16, 4, device="cpu")
+    cache.device = 3
     step = kq.Kv8Step(1, 3, torch.zeros(1, 2, dtype=torch.int32), 16)
     one, row = torch.zeros(1, dtype=torch.int32), torch.zeros(3, 1, 64)
     calls = {"plan": lambda: cache.plan(step, one, one, one, one, one), "append": lambda: cache.append(step, row, row),
@@ -48,8 +50,8 @@ def test_calls_in_the_order_of_torch(kq, monkeypatch, torch_stream, library):
         log.clear()
         call()
         only = [("call", "kq_b200_kv8_" + name)]
-        same = (torch_stream or 1) == library
-        assert log == (only if same else [(library, "waits for", torch_stream), *only, (torch_stream, "waits for", library)])
+        here = torch_stream or 1   # CUDA's name of the default stream
+        assert log == (only if here == library else [(library, "waits for", here), *only, (here, "waits for", library)])
 
 
 def test_set_stream_names_the_default_stream(kq, monkeypatch):
@@ -57,6 +59,6 @@ def test_set_stream_names_the_default_stream(kq, monkeypatch):
     log = []
     real = kq.lib()
     monkeypatch.setattr(kq, "lib", lambda: Library(real, log, 7))
-    for stream in (None, Stream(log, 0), Stream(log, 5)):
+    for stream in (None, Stream(0), Stream(5)):
         kq.set_stream(stream)
     assert log == [("set", None), ("set", 1), ("set", 5)]
