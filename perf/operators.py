@@ -6,6 +6,7 @@ result from elementary torch operations.  Both work on the state ``prepare``
 makes: the cache's code and scale arrays in the library's page layout, the
 block table and the step arrays of a ragged batch.
 """
+import ctypes
 import math
 import random
 import sys
@@ -282,6 +283,9 @@ def _handles(state):
     """What a user's program keeps from step to step: the cache over its arrays and the step's buffers."""
     if "cache" not in state:
         kq, c = _kqb200(), state["case"]
+        # the calls belong between torch's operations: one stream for both (1: CUDA's name of the default stream)
+        d = kq.abi.Diagnostic()
+        kq.abi.check(kq.lib().kq_b200_set_stream(torch.cuda.current_stream().cuda_stream or 1, ctypes.byref(d)), d)
         state["cache"] = kq.Kv8Cache(c["kv_heads"], c["head_dim"], c["page_tokens"], state["pages"], c["format"],
                                      codes=state.get("codes"), scales=state.get("scales"))
         step = kq.Kv8Step(c["requests"], state["tokens"], state["table"], c["page_tokens"])
