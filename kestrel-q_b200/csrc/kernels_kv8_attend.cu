@@ -778,14 +778,15 @@ Kv8Shape kv8_attend_shape(const Kv8Cache &c, const Kv8Step &s, uint32_t query_he
                           uint64_t max_kv_length) {
     Kv8Shape h{};
     const uint64_t G = query_heads / c.heads;
-    const uint64_t room = (uint64_t)s.columns * c.page_tokens;
+    // lengths are 32-bit: no request has more, however wide the table
+    const uint64_t room = std::min<uint64_t>((uint64_t)s.columns * c.page_tokens, INT32_MAX);
     const uint64_t deepest = max_kv_length == 0 ? room : std::min<uint64_t>(max_kv_length, room);
     const uint64_t groups = std::max<uint64_t>(1, ceil_div(deepest, kG));
     // the longest request, if every request brings a token
     const uint64_t longest = (s.tokens > s.requests ? s.tokens - s.requests : 0) + 1, rows = longest * G;
-    // 16-row groups that the row kernel would walk if it took everything
-    const uint64_t units = ceil_div((uint64_t)s.tokens * G, 16) * c.heads * groups;
-    const bool prompts = rows > kShortRows && units > kFewUnits;
+    // 16-row groups that the row kernel would walk if it took everything: strips * groups
+    const uint64_t strips = ceil_div((uint64_t)s.tokens * G, 16) * c.heads;
+    const bool prompts = rows > kShortRows && strips > kFewUnits / groups;
     h.row_limit = prompts ? kShortRows : UINT32_MAX;
     h.row_tile = rows <= 8 ? 8 : 16;
     // one wave of the row kernel, or shares of at least kMinShare groups

@@ -188,3 +188,25 @@ def test_reference_rounds_like_the_format():
     assert np.array_equal(ref.encode(mid, "e4m3"), even.astype(np.float32))
     assert np.array_equal(ref.encode(-mid, "e4m3"), -even.astype(np.float32))
     assert np.array_equal(ref.encode(np.float32([0.5, 1.5, -2.5, 126.6, 200]), "int8"), np.float32([0, 2, -2, 127, 127]))
+
+
+@pytest.mark.parametrize("columns", [1 << 28, 1 << 29, 3 << 29, (1 << 32) - 1])
+@pytest.mark.parametrize("tokens", [1, 100, 800, 1600, 2400, 6000])
+def test_attention_workspace_of_the_widest_tables(kq, columns, tokens):
+    """A request has 2^31 - 1 tokens at most, whatever its row of the table
+    could hold: tables past that are cut like one that holds as many."""
+    def size(columns):
+        n = C.c_uint64(1)
+        s = _step(kq, token_capacity=tokens, table_columns=columns, table_stride=columns)
+        assert _call(kq, "kq_b200_kv8_attend_workspace_bytes", _cache(kq, page_tokens=128), s, 8, 0, C.byref(n)) == 0
+        return n.value
+    assert size(columns) == size((1 << 31) // 128)
+
+
+def test_attention_of_the_largest_counts(kq):
+    """1024 heads, 2^31 rows a head and the longest contexts: the launch rule's
+    products pass 2^64, and the step is too large, not small."""
+    n = C.c_uint64(1)
+    c = _cache(kq, kv_head_count=1024, page_tokens=128)
+    s = _step(kq, request_count=1, token_capacity=(1 << 31) - 1, table_columns=1 << 25, table_stride=1 << 25)
+    assert _call(kq, "kq_b200_kv8_attend_workspace_bytes", c, s, 1024, 0, C.byref(n)) == kq.abi.LIMIT_EXCEEDED
