@@ -586,11 +586,12 @@ void kq_b200_profile_read(uint64_t *launches, double *total_ms);
  *   kq_b200_kv8_attend  causal attention of the new tokens over the pages
  *   kq_b200_kv8_read    the values that pages hold
  *
- * All arrays are device memory of the current device.  The calls are
- * asynchronous on the library stream; what is wrong in the arrays' contents
- * (lengths, page ids and slots out of range: KQ_STATUS_SPAN_OUT_OF_RANGE;
- * non-finite values: KQ_STATUS_NUMERIC_DOMAIN) surfaces at
- * kq_b200_synchronize, and nothing is read or written out of range meanwhile.
+ * All arrays are device memory of the current device, aligned to their
+ * values at least.  The calls are asynchronous on the library stream; what is
+ * wrong in the arrays' contents (lengths, page ids and slots out of range:
+ * KQ_STATUS_SPAN_OUT_OF_RANGE; non-finite values: KQ_STATUS_NUMERIC_DOMAIN)
+ * surfaces at kq_b200_synchronize, and nothing is read or written out of range
+ * meanwhile.
  * After such an error the outputs of the failing call, and of the calls after
  * it up to the synchronize, are unspecified; pages that a failed append met
  * hold either their old rows or the new ones. */

@@ -45,6 +45,15 @@ bool any_missing(const Span (&spans)[N]) {
     return false;
 }
 
+// Every array holds values of 4 bytes or more (what needs more alignment is
+// checked where it is known).
+template <size_t N>
+bool any_misaligned(const Span (&spans)[N]) {
+    for (const Span &s : spans)
+        if (!aligned(s.p, 4)) return true;
+    return false;
+}
+
 template <size_t N, size_t M>
 bool any_overlap(const Span (&writes)[N], const Span (&reads)[M]) {
     for (size_t i = 0; i < N; ++i) {
@@ -196,6 +205,8 @@ kq_status kq_b200_kv8_plan(const kq_b200_kv8_cache *cache, const kq_b200_kv8_ste
     if (s.runs == 0 || any_missing(writes) || any_missing(reads))
         return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "a plan takes lengths, a free list and every array of the step");
     if (!aligned(s.slots, 8)) return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "slots need 8-byte alignment");
+    if (any_misaligned(writes) || any_misaligned(reads))
+        return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "arrays need 4-byte alignment");
     if (any_overlap(writes, reads))
         return fail(diagnostic, KQ_STATUS_ALIASING_VIOLATION, "a plan's outputs must not overlap each other or its inputs");
     DeviceContext *ctx;
@@ -229,6 +240,8 @@ kq_status kq_b200_kv8_append(const kq_b200_kv8_cache *cache, const kq_b200_kv8_s
     if (s.runs == 0 || any_missing(reads))
         return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT, "an append takes key and value rows, slots and page runs");
     if (!aligned(s.slots, 8)) return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "slots need 8-byte alignment");
+    if (any_misaligned(writes) || any_misaligned(reads))
+        return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "arrays need 4-byte alignment");
     if (any_overlap(writes, reads))
         return fail(diagnostic, KQ_STATUS_ALIASING_VIOLATION, "cache arrays must not overlap each other or the rows");
     DeviceContext *ctx;
@@ -255,6 +268,8 @@ kq_status kq_b200_kv8_read(const kq_b200_kv8_cache *cache, const int32_t *pages,
     const Span writes[] = {{values, want * 4}};
     const Span reads[] = {{c.codes, kq_b200_kv8_codes_bytes(cache)}, {c.scales, 4 * kq_b200_kv8_scales_count(cache)},
                           {pages, 4ull * count}};
+    if (any_misaligned(writes) || any_misaligned(reads))
+        return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "arrays need 4-byte alignment");
     if (any_overlap(writes, reads))
         return fail(diagnostic, KQ_STATUS_ALIASING_VIOLATION, "values must not overlap the cache or the page ids");
     DeviceContext *ctx;
@@ -319,6 +334,8 @@ kq_status kq_b200_kv8_attend(const kq_b200_kv8_cache *cache, const kq_b200_kv8_s
     if (any_missing(writes) || any_missing(reads))
         return fail(diagnostic, KQ_STATUS_INVALID_ARGUMENT,
                     "attention takes queries, an output, a block table, query offsets and lengths");
+    if (any_misaligned(writes) || any_misaligned(reads))
+        return fail(diagnostic, KQ_STATUS_INVALID_ALIGNMENT, "arrays need 4-byte alignment");
     if (any_overlap(writes, reads))
         return fail(diagnostic, KQ_STATUS_ALIASING_VIOLATION, "attention outputs must not overlap each other or its inputs");
     DeviceContext *ctx;

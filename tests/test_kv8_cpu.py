@@ -210,3 +210,20 @@ def test_attention_of_the_largest_counts(kq):
     c = _cache(kq, kv_head_count=1024, page_tokens=128)
     s = _step(kq, request_count=1, token_capacity=(1 << 31) - 1, table_columns=1 << 25, table_stride=1 << 25)
     assert _call(kq, "kq_b200_kv8_attend_workspace_bytes", c, s, 1024, 0, C.byref(n)) == kq.abi.LIMIT_EXCEEDED
+
+
+def test_refused_alignment_of_small_arrays(kq):
+    """Arrays of 4-byte values at odd addresses: a kernel that read them would fault."""
+    a = kq.abi
+    arrays = {n: A + (i + 2 << 30) + 2 for i, n in enumerate(
+        ["block_table", "query_offsets", "kv_lengths", "slots", "positions", "run_offsets", "page_runs"])}
+    for n, p in arrays.items():
+        assert plan(kq, step=_step(kq, **{n: p})) == a.INVALID_ALIGNMENT, n
+    for n, p in dict(ctx=CTX, new=NEW, free=FREE, head=HEAD, head_out=HEAD_OUT).items():
+        assert plan(kq, **{n: p + 2}) == a.INVALID_ALIGNMENT, n
+    for n in ("slots", "page_runs"):
+        assert append(kq, step=_step(kq, **{n: arrays[n]})) == a.INVALID_ALIGNMENT, n
+    for n in ("block_table", "query_offsets", "kv_lengths"):
+        assert attend(kq, step=_step(kq, **{n: arrays[n]})) == a.INVALID_ALIGNMENT, n
+    assert attend(kq, lse=LSE + 2) == a.INVALID_ALIGNMENT
+    assert read(kq, pages=CTX + 1) == a.INVALID_ALIGNMENT
