@@ -130,10 +130,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 //   p sV 2^(6 - z),   p = 2^(l - m)
 // at most 2^14; it loses bits only where it is small beside the row's largest
 // p sV, however large the values that the row does not attend to.  Either point
-// moves when it is 8 below a step's largest.  Scales below 2^-80 count as that,
-// which bounds z from below; sV 2^(6 - z) can only overflow (scales from 2^33,
-// beside such small ones) where p is below 2^-114, and stays finite then.
-__device__ __forceinline__ float size_of(float scale) { return fmaxf(__log2f(scale), -80.0f); }
+// moves when it is 8 below a step's largest.  Scales below 2^-110 count as that:
+// z, at most 9 below them, keeps 2^(6 - z) and 2^(z - 6) normal numbers.  A
+// page of scale 2^-119 still has 22 bits (weights of 2^-2 and more), one of
+// 2^-136 counts as zeros.  sV 2^(6 - z) can overflow only where p is below
+// 2^-114 (p sV is 2^(z + 8) at most), and stays finite then.
+__device__ __forceinline__ float size_of(float scale) { return fmaxf(__log2f(scale), -110.0f); }
 __device__ __forceinline__ float weight_of(float m, float z) {   // of p sV
     return m == -INFINITY ? 0.0f : exp2_approx(kWeightBits - z);
 }

@@ -522,7 +522,10 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 ok = bar_wait_warp(&sh.back[m], 0, quit);
             }
             if (ok) {
-                if (whole) scale *= sum > 0.0f ? 1.0f / sum : 0.0f;
+                // to units of 2^m, then by the sum: in one factor, except where that
+                // would leave F32's normal numbers (small values)
+                float inv = !whole ? 1.0f : sum > 0.0f ? 1.0f / sum : 0.0f;
+                if (z > -64.0f) scale *= inv, inv = 1.0f;
                 bool fine = sum < INFINITY;
                 const uint64_t to = row_out(row);
 #pragma unroll 1
@@ -538,8 +541,8 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                     if (!live) continue;
 #pragma unroll
                     for (int g = 0; g < 32; g += 4) {
-                        const float4 o = make_float4(__uint_as_float(x[g]) * scale, __uint_as_float(x[g + 1]) * scale,
-                                                     __uint_as_float(x[g + 2]) * scale, __uint_as_float(x[g + 3]) * scale);
+                        const float4 o = make_float4(__uint_as_float(x[g]) * scale * inv, __uint_as_float(x[g + 1]) * scale * inv,
+                                                     __uint_as_float(x[g + 2]) * scale * inv, __uint_as_float(x[g + 3]) * scale * inv);
                         fine &= fabsf(o.x) + fabsf(o.y) + fabsf(o.z) + fabsf(o.w) < INFINITY;
                         if (whole)
                             store4<BF16>(a.out, to + n + g, o);
