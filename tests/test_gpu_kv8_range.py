@@ -42,3 +42,29 @@ def test_attention_over_small_values(kq, dtype, dim, new, value):
     assert seen.count == (new > 1)
     o = check(s, n, new, G, q, float(np.float32(dim ** -0.5)), got)
     assert np.all(o.any(-1))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 300])
+def test_small_values_are_ordinary_ones_scaled(kq, dtype, dim, new):
+    """Values 2^-100 times others give 2^-100 times their output, to the bit:
+    every factor between them is a power of two while nothing is subnormal.
+    The page scales are 2^-109, and the weights, up to 2^7.8 above a reference
+    point that the first 128 tokens set, add up to 2^17."""
+    n, G = 500, 3
+    got = []
+    for size in (0.25, 0.25 * 2.0 ** -100):
+        s = Server(kq, 1, dim, 16, "int8", 1, 210, pages=60, dtype=dtype, seed=dim)
+        k = np.zeros((800, 1, dim), np.float32)
+        k[128:, 0, 0] = 5.4
+        v = (np.float32(size) * s.rng.uniform(0.5, 1, (800, 1, dim)).astype(np.float32))
+        s.step([n], k=k[:n], v=v[:n])
+        step = s.step([new], k=k[n:n + new], v=v[n:n + new])
+        q = np.zeros((new, G, dim), np.float32)
+        q[:, :, 0] = 1
+        with Launches(kq, "kv8_prompt") as seen:
+            got.append(s.attend(step, [new], G, q=q, scale=1.0, check=False))
+        assert seen.count == (new > 1)
+    assert np.array_equal(got[0][0], got[1][0] * np.float32(2.0 ** 100)) and np.all(got[0][0] > 0.1)
+    assert np.array_equal(got[0][1], got[1][1])
