@@ -593,8 +593,11 @@ void kq_b200_profile_read(uint64_t *launches, double *total_ms);
  * surfaces at kq_b200_synchronize, and nothing is read or written out of range
  * meanwhile.
  * After such an error the outputs of the failing call, and of the calls after
- * it up to the synchronize, are unspecified; pages that a failed append met
- * hold either their old rows or the new ones. */
+ * it up to the synchronize, are unspecified; of a page that a failed append
+ * met, each head's keys, and each head's values, are as they were or as the
+ * append makes them (rows of the page's last owner among them, where the run
+ * begins it).  The append can be made again, with finite rows, and then gives
+ * what it would have given. */
 typedef enum kq_b200_kv8_format {
     KQ_B200_KV8_INT8 = 0, /* -127 .. 127 */
     KQ_B200_KV8_E4M3      /* 8-bit float, largest value 448 */
@@ -677,8 +680,9 @@ kq_status kq_b200_kv8_plan(const kq_b200_kv8_cache *cache,
  * held divided by 127 (int8) or 448 (e4m3): where new rows exceed it, the
  * rows before them are rounded again to the new scale.  A run that begins at
  * a page's first row starts the page anew and clears the rows behind it; rows
- * behind a run that begins later stay as they are.  Non-finite rows leave
- * their page as it was.  The runs of a call must lie in different pages (as
+ * behind a run that begins later keep their codes.  A non-finite value leaves
+ * its head's keys, or values, of the page as they were (the other heads' may
+ * be new).  The runs of a call must lie in different pages (as
  * kq_b200_kv8_plan makes them): what two runs in one page leave there is
  * unspecified. */
 kq_status kq_b200_kv8_append(const kq_b200_kv8_cache *cache,
