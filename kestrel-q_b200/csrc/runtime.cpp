@@ -174,14 +174,15 @@ kq_status DeviceContext::synchronize(kq_diagnostic *d) {
     if (word != 0ull) {
         uint32_t failing = (uint32_t)(word & 0xffffffffull);
         uint32_t code = (uint32_t)(word >> 32);
+        const bool states = !dirty.empty();   // else the calls since the last synchronize advanced none
         for (Rollbackable *r : dirty) r->on_error(failing);
         dirty.clear();
         KQB_CUDA(cudaMemsetAsync(err_word, 0, sizeof(unsigned long long), stream), d, "error word reset");
         kq_status s = code == kErrSelection ? KQ_STATUS_INVALID_QSA_STATE
                       : code == kErrStep    ? KQ_STATUS_SPAN_OUT_OF_RANGE
                                             : KQ_STATUS_NUMERIC_DOMAIN;
-        diag_set(d, s, "device reported %s (code 0x%x, call %u); state rolled back", error_text(code), code,
-                 failing);
+        diag_set(d, s, "device reported %s (code 0x%x, call %u)%s", error_text(code), code, failing,
+                 states ? "; state rolled back" : "");
         return s;
     }
     for (Rollbackable *r : dirty) r->on_success();

@@ -48,3 +48,17 @@ def test_pages_of_a_failed_append(kq, fmt, at):
     s.cache.append(step, k, v)
     kq.synchronize()
     s.check_pages()
+
+
+@pytest.mark.parametrize("what", ["length", "row"])
+def test_error_text_of_cache_calls(kq, what):
+    """No state is rolled back for a cache call, and the text does not say so."""
+    import torch
+    s = Server(kq, 1, 64, 16, "int8", 1, 2)
+    step = kq.Kv8Step(1, 3, s.table_dev, 16)
+    s.cache.plan(step, *(dev(np.int32(a)) for a in ([0], [-1 if what == "length" else 3], s.free, [0], [0])))
+    s.cache.append(step, torch.full((3, 1, 64), math.inf, device="cuda"), torch.zeros(3, 1, 64, device="cuda"))
+    with pytest.raises(kq.KQError) as e:
+        kq.synchronize()
+    assert e.value.status == (kq.abi.SPAN_OUT_OF_RANGE if what == "length" else kq.abi.NUMERIC_DOMAIN)
+    assert "device reported" in str(e.value) and "rolled back" not in str(e.value)
