@@ -366,8 +366,10 @@ kq_status kq_b200_order_stream(void *cuda_stream, int library_first, kq_diagnost
     const cudaStream_t other = static_cast<cudaStream_t>(cuda_stream);
     if (other == c->stream) return KQ_STATUS_OK;
     const cudaEvent_t event = c->order[library_first != 0];
-    KQB_CUDA(cudaEventRecord(event, library_first ? c->stream : other), diagnostic, "stream order record");
-    KQB_CUDA(cudaStreamWaitEvent(library_first ? other : c->stream, event, 0), diagnostic, "stream order wait");
+    cudaError_t e = cudaEventRecord(event, library_first ? c->stream : other);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(library_first ? other : c->stream, event, 0);
+    if (e != cudaSuccess) cudaGetLastError();   // not the next launch's error
+    KQB_CUDA(e, diagnostic, "stream order");
     return KQ_STATUS_OK;
 }
 
