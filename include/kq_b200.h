@@ -703,7 +703,12 @@ kq_status kq_b200_kv8_read(const kq_b200_kv8_cache *cache,
                            uint64_t values_capacity,
                            kq_diagnostic *diagnostic);
 
-/* Work space that kq_b200_kv8_attend needs for these sizes (0: none). */
+/* Work space that kq_b200_kv8_attend needs for these sizes (0: none).  It goes
+ * by the capacities: where token_capacity leaves room for a request of more
+ * than 64 query rows per key/value head, tiles of such rows are set aside for
+ * every request.  A decode step of token_capacity = request_count needs some
+ * MB; 64 requests of 16 / 2 heads of 256 over tables of 32k tokens 531 MB with
+ * 8 tokens more. */
 kq_status kq_b200_kv8_attend_workspace_bytes(const kq_b200_kv8_cache *cache,
                                              const kq_b200_kv8_step *step,
                                              uint32_t query_heads,
@@ -720,10 +725,16 @@ kq_status kq_b200_kv8_attend_workspace_bytes(const kq_b200_kv8_cache *cache,
  * (natural logarithm, [token][query heads], may be NULL).  A row that sees
  * nothing gets zeros and -infinity; rows behind the last request are left as
  * they were.  Uses step->block_table, query_offsets and kv_lengths only.
- * Query and output have the same type; products are exact in the codes and
- * hold 22 bits of an F32 query, sums and the softmax are F32.  Weights are not
- * normalised before they are summed: values of 2^100 and more can leave F32's
- * range in long sums, which is reported like other non-finite values.
+ * Query and output have the same type.  Products are exact in the codes and
+ * hold 22 bits of an F32 query; weights enter the second product with 22 bits
+ * for F32 outputs and with 11 for bf16 ones (2^-11 relative to each weight,
+ * beside 2^-8 of the output's own rounding); sums and softmax statistics are
+ * F32, the sums those of tensor cores, which truncate (F32 prompts: over 512
+ * tokens at a time).  Weights are not normalised before they are summed: values
+ * of 2^100 and more can leave F32's range in long sums, which is reported like
+ * other non-finite values.  At the other end, query rows whose largest element
+ * is below 2^-115 and value scales below 2^-119 (bf16: 2^-130) lose bits, value
+ * scales of 2^-142 count as 0, and weights below 2^-114 of a row's largest may.
  * `max_kv_length` (0: what the table's columns hold) and the capacities only
  * decide how the work is cut; the result is right for any lengths, and the
  * same for the same cut.  `workspace` is private to the call until it has

@@ -132,8 +132,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // p sV, however large the values that the row does not attend to.  Either point
 // moves when it is 8 below a step's largest.  Scales below 2^-110 count as that:
 // z, at most 9 below them, keeps 2^(6 - z) and 2^(z - 6) normal numbers.  A
-// page of scale 2^-119 still has 22 bits (weights of 2^-2 and more), one of
-// 2^-136 counts as zeros.  sV 2^(6 - z) can overflow only where p is below
+// page of scale 2^-119 still has 22 bits (weights of 2^-3 and more), one of
+// 2^-142 counts as zeros.  sV 2^(6 - z) can overflow only where p is below
 // 2^-114 (p sV is 2^(z + 8) at most), and stays finite then.
 __device__ __forceinline__ float size_of(float scale) { return fmaxf(__log2f(scale), -110.0f); }
 __device__ __forceinline__ float weight_of(float m, float z) {   // of p sV

@@ -16,8 +16,8 @@
 // 2^-27 below the row's largest lose bits, below F32's own rounding of the
 // sum), F32 queries are split into two fp16 parts (22 bits).  P sV is scaled
 // into fp16's range the same way (below) and split in two for F32 outputs;
-// for bfloat16 outputs one part is kept: 11 bits, 2^-12 relative per weight
-// against the output's own 2^-9.  The page scales multiply the accumulators
+// for bfloat16 outputs one part is kept: 11 bits, 2^-11 relative per weight
+// against the output's own 2^-8.  The page scales multiply the accumulators
 // (sK) and the weights (sV), never the codes.
 //
 // Softmax in base 2, one pass: a row's reference point m is raised only when
@@ -712,14 +712,30 @@ kv8_prompt_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, Error
 namespace {
 
 constexpr uint32_t kSms = 148;
-constexpr uint32_t kShortRows = 64;        // requests up to this many rows go to the row kernel
-// Steps of at most this many units go to the row kernel whole: a prompt tile
-// takes 19 us at least, the row kernel 8 us and about 1.7 ns a unit (7 odd
-// requests, 37 tokens over 333, 10 heads of 64: 27 us in both kernels, 12 in
-// the row kernel alone).
+// Requests of up to this many rows go to the row kernel.  8 requests over 8k
+// cached tokens, row / prompt kernel: F32, 2 heads of 256: 64 rows 88 / 100 us,
+// 128 rows 143 / 107; bf16, 8 heads of 128: 119 / 170 and 213 / 178.
+constexpr uint32_t kShortRows = 64;
+// Steps of at most this many units (as the launch sees them: capacities, not
+// lengths) go to the row kernel whole: a prompt tile takes 19 us at least, the
+// row kernel 8 us and about 1.7 ns a unit.  Two chunks over 256, 1k, 4k and 8k
+// cached tokens, row / prompt kernel: F32, 24 tokens, 2 heads of 256 (960, 3264,
+// 12480, 24768 units) 27 / 43, 31 / 88, 47 / 90, 70 / 96 us; bf16, 40 tokens, 8
+// heads of 128 over 256, 1k, 4k (3200, 10880, 41600) 20 / 35, 29 / 57, 51 / 61.
+// With so few tiles the row kernel is ahead past the limit too; with many it is
+// not (8 requests of 128 rows, 65920 units: 143 / 107).
 constexpr uint64_t kFewUnits = 8192;
-constexpr uint32_t kManyPartials = 8;      // shares per tile from which a tile is joined by many CTAs
-constexpr uint32_t kMinPromptGroups = 64;  // a split of a prompt: 1024 tokens or more
+// Shares per tile from which a tile is joined by many CTAs.  Many / one, F32, 2
+// heads of 256: one request of 4k, 32k, 131k tokens (32, 222, 222 shares a tile)
+// 16 / 22, 25 / 61, 45 / 82 us; 8, 16, 32 of 8k (28, 14, 7) 37 / 39, 53 / 49,
+// 84 / 72; bf16, 8 heads of 128: 8 of 8k (9) 49 / 45.
+constexpr uint32_t kManyPartials = 8;
+// A split of a prompt: this many groups (1024 tokens) or more.  One F32 request,
+// 2 heads of 256, with 16, 32, 64 and 256: 128 tokens over 2k 57, 61, 90, 145 us;
+// over 16k 205, 205, 180, 250; bf16, 8 heads of 128, 32 tokens over 4k 45, 45,
+// 53, 123; over 16k 84, 84, 61, 124: short splits win over short contexts, and
+// lose to their joins over long ones.
+constexpr uint32_t kMinPromptGroups = 64;
 
 template <int D, int NT, bool BF16, bool E4M3>
 void launch_rows(const Kv8Cache &c, const Kv8Step &s, const Kv8Attend &a, const Kv8Shape &h, ErrorWord err,
