@@ -757,9 +757,10 @@ kv8_prompt_kernel(Kv8Cache c, Kv8Step s, Kv8Attend a, Kv8Shape shape, ErrorWord 
                 }
             }
         }
-        // nothing of this CTA's is in flight after this
+        // nothing of this CTA's is in flight after this; the abort flag does not
+        // cut this wait short
         umma_commit(&sh.drained);
-        bar_wait(&sh.drained, 0, quit);
+        if (!bar_wait(&sh.drained, 0)) *quit = 1;
     }
     __syncwarp();
     fence_before();
