@@ -585,27 +585,6 @@ def set_stream(stream=None) -> None:
     abi.check(lib().kq_b200_set_stream(None if stream is None else stream.cuda_stream or 1, C.byref(d)), d)
 
 
-def _in_order(device: int | None, call, *args) -> None:
-    """`call` in the order of torch's current stream on CUDA device `device`:
-    after what that stream holds, and before what it is given next (so memory
-    that torch reuses on it is no longer in use).  Two events, unless it is the
-    library stream (:func:`set_stream`).  Arrays on no CUDA device (None) are
-    the library's to refuse."""
-    import torch
-    library, d = lib(), abi.Diagnostic()
-    # the handle alone: torch.cuda.current_stream takes 2.6 us to make an object of it
-    here = None if device is None else torch._C._cuda_getCurrentRawStream(device) or 1
-    if here is None or here == library.kq_b200_get_stream():
-        abi.check(call(*args, C.byref(d)), d)
-        return
-    abi.check(library.kq_b200_order_stream(here, 0, C.byref(d)), d)
-    status = call(*args, C.byref(d))
-    after = abi.Diagnostic()
-    ordered = library.kq_b200_order_stream(here, 1, C.byref(after))
-    abi.check(status, d)
-    abi.check(ordered, after)
-
-
 class Kv8Step:
     """The device arrays of one step of a paged cache (kq_b200_kv8_step):
     `requests` rows of `block_table` (int32 [requests][columns], the caller's),
@@ -669,8 +648,27 @@ class Kv8Cache:
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("cache arrays must be contiguous")
         self.device = codes.device.index   # None: not a CUDA device
+        # the handle alone: torch.cuda.current_stream takes 2.6 us to make an object of it
+        self._stream = torch._C._cuda_getCurrentRawStream
         self.args.codes, self.args.codes_bytes = codes.data_ptr(), codes.numel()
         self.args.scales, self.args.scales_count = scales.data_ptr(), scales.numel()
+
+    def _run(self, call, *args) -> None:
+        """`call` in the order of torch's current stream: after what that stream
+        holds, and before what it is given next (so memory that torch reuses on
+        it is no longer in use).  Two events, unless it is the library stream
+        (:func:`set_stream`).  Arrays on no CUDA device are the library's to refuse."""
+        library, d = lib(), abi.Diagnostic()
+        here = None if self.device is None else self._stream(self.device) or 1
+        if here is None or here == library.kq_b200_get_stream():
+            abi.check(call(*args, C.byref(d)), d)
+            return
+        abi.check(library.kq_b200_order_stream(here, 0, C.byref(d)), d)
+        status = call(*args, C.byref(d))
+        after = abi.Diagnostic()
+        ordered = library.kq_b200_order_stream(here, 1, C.byref(after))
+        abi.check(status, d)
+        abi.check(ordered, after)
 
     def _rows(self, name: str, a, tokens: int, heads: int | None):
         """(dtype, address, token stride) of rows [tokens][heads][head_dim]
@@ -690,7 +688,7 @@ class Kv8Cache:
         for a, least in ((context_lengths, n), (new_lengths, n), (free_pages, 0), (free_head, 1), (free_head_out, 1)):
             if a.dtype != self._int32 or a.numel() < least or not a.is_contiguous():
                 raise ValueError("a plan takes consecutive int32 lengths, free pages and heads")
-        _in_order(self.device, lib().kq_b200_kv8_plan, self.args, step.args, context_lengths.data_ptr(),
+        self._run(lib().kq_b200_kv8_plan, self.args, step.args, context_lengths.data_ptr(),
                   new_lengths.data_ptr(), free_pages.data_ptr(), free_pages.numel(), free_head.data_ptr(),
                   free_head_out.data_ptr())
 
@@ -701,13 +699,13 @@ class Kv8Cache:
         vt, vp, vs = self._rows("value", value, n, self.kv_heads)
         if kt != vt:
             raise ValueError("key and value must have the same type")
-        _in_order(self.device, lib().kq_b200_kv8_append, self.args, step.args, kt, kp, ks, vp, vs)
+        self._run(lib().kq_b200_kv8_append, self.args, step.args, kt, kp, ks, vp, vs)
 
     def read_pages(self, pages, values) -> None:
         """values (float32 [pages][heads][key, value][page_tokens][head_dim]) of the page ids `pages` (int32)."""
         if pages.dtype != self._int32 or values.dtype != self._float32 or not (pages.is_contiguous() and values.is_contiguous()):
             raise ValueError("contiguous int32 pages and float32 values are required")
-        _in_order(self.device, lib().kq_b200_kv8_read, self.args, pages.data_ptr(), pages.numel(), values.data_ptr(),
+        self._run(lib().kq_b200_kv8_read, self.args, pages.data_ptr(), pages.numel(), values.data_ptr(),
                   values.numel())
 
     def attend_workspace_bytes(self, step: Kv8Step, query_heads: int, max_kv_length: int = 0) -> int:
@@ -731,7 +729,7 @@ class Kv8Cache:
                 raise ValueError("lse: one float32 per token and query head is required")
         if workspace is not None and not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        _in_order(self.device, lib().kq_b200_kv8_attend, self.args, step.args, qt, qp, qs, query.shape[1], scale,
+        self._run(lib().kq_b200_kv8_attend, self.args, step.args, qt, qp, qs, query.shape[1], scale,
                   max_kv_length, op, os, None if lse is None else lse.data_ptr(),
                   None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes)
 
