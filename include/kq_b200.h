@@ -440,7 +440,7 @@ void *kq_b200_get_stream(void);
  * waiting on the host: on the library stream behind `cuda_stream`, a stream of
  * the current device (NULL: the legacy default stream), or with library_first
  * the other way round.  Can be captured: the later stream joins the earlier
- * one's capture. */
+ * one's capture, as do other threads' calls on it until the capture ends. */
 kq_status kq_b200_order_stream(void *cuda_stream, int library_first, kq_diagnostic *diagnostic);
 
 /* One decode token for each of `batch` independent sequences.
